@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+from contextlib import nullcontext
 from ctypes import c_char_p, c_int, c_int64, c_size_t, c_void_p
 
 import torch
@@ -57,6 +58,11 @@ SIGNATURES = {
     "fr_gather_rows": (_I, [_P, _L, _P, _L, _I, _P, _L, _P]),
     "fr_w4a16_gemm": (_I, [_P, _L, _P, _P, _P, _L, _I, _I, _I, _P, _L, _I, _P]),
     "fr_w4a16_dequant": (_I, [_P, _P, _P, _I, _I, _I, _P, _L, _P]),
+    "fr_fp4_quantize_workspace_bytes": (_Z, [_L, _L, _L]),
+    "fr_fp4_quantize": (_I, [_P, _I, _L, _L, _L, _L, _L, _I, _P, _I, _P, _P, _P, _Z, _P]),
+    "fr_fp4_dequantize": (_I, [_P, _P, _P, _L, _L, _L, _I, _I, _P, _P]),
+    "fr_moe_decode_workspace_bytes": (_Z, [_L, _I, _I, _I, _I]),
+    "fr_moe_decode": (_I, [_P, _P, _L, _L, _P, _P, _P, _P, _P, _P, _I, _I, _L, _I, _I, _I, _I, _I, _P, _P, _P, _P, _Z, _P]),
 }
 
 _lib = None
@@ -112,6 +118,20 @@ def require_cuda(*tensors) -> None:
             raise FastRouteError("fast_route_b200 runs on CUDA tensors only; there is no CPU path")
 
 
+def require_device(device, *tensors) -> None:
+    """All tensors of a call on one GPU."""
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise FastRouteError(f"tensors on different devices: {t.device} and {device}")
+
+
+def on_device(device):
+    """Makes ``device`` the current one for a call (kernels launch on the current device)."""
+    if torch.cuda.current_device() == device.index:
+        return nullcontext()
+    return torch.cuda.device(device)
+
+
 def device_status():
     """Synchronises and returns (code, detail, block, count) of the device status block."""
     out = (ctypes.c_uint * 4)()
@@ -139,5 +159,15 @@ def workspace(nbytes: int, device, tag: str = "layer") -> torch.Tensor:
     if buf is None or buf.numel() < nbytes + 1024:
         buf = torch.zeros(int(nbytes) + 1024, dtype=torch.uint8, device=device)
         _workspaces[key] = buf
+    off = (-buf.data_ptr()) % 1024
+    return buf[off:off + max(nbytes, 1)]
+
+
+def call_workspace(nbytes: int, device, tag: str) -> torch.Tensor:
+    """``workspace`` for calls that may be captured: inside a stream capture every call gets zeroed memory of its own
+    from the graph's pool, so that two graphs replayed side by side share none.  ``device`` is the current one."""
+    if not torch.cuda.is_current_stream_capturing():
+        return workspace(nbytes, device, tag)
+    buf = torch.zeros(int(nbytes) + 1024, dtype=torch.uint8, device=device)
     off = (-buf.data_ptr()) % 1024
     return buf[off:off + max(nbytes, 1)]

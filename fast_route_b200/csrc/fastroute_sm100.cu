@@ -6,4 +6,6 @@
 #include "fr_gemm_tokenn.cu"
 #include "fr_w4a16.cu"
 #include "fr_ep.cu"
+#include "fr_fp4.cu"
+#include "fr_decode.cu"
 #include "fr_api.cu"

@@ -1466,4 +1466,35 @@ int fr_moe_experts(const void* rows, const int32_t* row_expert, const float* row
                       static_cast<cudaStream_t>(stream));
 }
 
+size_t fr_fp4_quantize_workspace_bytes(int64_t mats, int64_t rows, int64_t cols) {
+  return fr::fp4_quantize_workspace(mats, rows, cols);
+}
+
+int fr_fp4_quantize(const void* x, int dtype, int64_t mats, int64_t rows, int64_t cols, int64_t ld_mat, int64_t ld_row,
+                    int block, float* global_scale, int own_global, void* q, void* scale, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  return fr::fp4_quantize_dispatch(x, dtype, mats, rows, cols, ld_mat, ld_row, block, global_scale, own_global, q, scale,
+                                   workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int fr_fp4_dequantize(const void* q, const void* scale, const float* global_scale, int64_t mats, int64_t rows,
+                      int64_t cols, int block, int dtype, void* out, void* stream) {
+  return fr::fp4_dequantize_dispatch(q, scale, global_scale, mats, rows, cols, block, dtype, out,
+                                     static_cast<cudaStream_t>(stream));
+}
+
+size_t fr_moe_decode_workspace_bytes(int64_t M, int H, int I, int E, int topk) {
+  return H > 0 ? fr::moe_decode_workspace(M, I, E, topk) : 0;
+}
+
+int fr_moe_decode(const void* x, const void* gate, int64_t gate_stride_h, int64_t gate_stride_e, const void* w1,
+                  const void* w1_scale, const float* w1_global, const void* w2, const void* w2_scale,
+                  const float* w2_global, int dtype, int block, int64_t M, int H, int I, int E, int topk,
+                  int renormalize, void* out, float* topk_weights_out, int32_t* topk_ids_out, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+  return fr::moe_decode_dispatch(x, gate, gate_stride_h, gate_stride_e, w1, w1_scale, w1_global, w2, w2_scale, w2_global,
+                                 dtype, block, M, H, I, E, topk, renormalize, out, topk_weights_out, topk_ids_out,
+                                 workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"

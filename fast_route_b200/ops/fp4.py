@@ -1,0 +1,99 @@
+"""Microscaled 4-bit floating point: E2M1 codes with a scale per block of 16 or 32 elements of a row.
+
+``block=16``: E4M3 block scales and one fp32 scale per matrix (``value = code * (scale * global)``);
+``block=32``: E8M0 block scales (powers of two, ``value = code * scale``).  Codes are packed two per byte, the even
+element in the low half.  The type of the scale tensor (``float8_e4m3fn`` / ``float8_e8m0fnu``) tells the two apart.
+The reference has no such format; its 4-bit weights are GPTQ integers (``ops/splitk_gemm.py``).
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+
+_SCALE_DTYPE = {16: torch.float8_e4m3fn, 32: torch.float8_e8m0fnu}
+
+
+def block_of(q: torch.Tensor, scale: torch.Tensor, what: str = "scale") -> int:
+    """The block size of a quantised matrix, after checking that codes and scales belong together."""
+    assert q.dtype == torch.uint8, "codes are packed in uint8"
+    assert scale.dtype in (torch.float8_e4m3fn, torch.float8_e8m0fnu), f"{what} must be float8_e4m3fn or float8_e8m0fnu"
+    block = 16 if scale.dtype == torch.float8_e4m3fn else 32
+    assert q.is_contiguous() and scale.is_contiguous(), f"codes and {what} must be contiguous"
+    assert scale.shape == (*q.shape[:-1], q.shape[-1] * 2 // block) and q.shape[-1] * 2 % block == 0, \
+        f"{what} does not match the codes"
+    return block
+
+
+def check_global(g: torch.Tensor, mats: int, block: int, what: str = "global_scale") -> None:
+    if g is None:
+        return
+    assert block == 16, f"{what} goes with block 16 only"
+    assert g.dtype == torch.float32 and g.numel() == mats and g.is_contiguous(), f"{what}: one fp32 number per matrix"
+
+
+def quantize_fp4(x: torch.Tensor, block: int = 16, global_scale: torch.Tensor = None):
+    """``x[rows, cols]`` or ``x[mats, rows, cols]`` (fp16, bf16 or fp32; any strides with adjacent elements in a row)
+    -> ``(q[..., cols/2] uint8, scale[..., cols/block], global_scale)``.
+
+    ``block=16``: ``global_scale`` (fp32, one per matrix) is computed from the largest magnitude, or taken from the
+    caller (a calibrated value: one pass over ``x`` less) and returned as given.  ``block=32`` has none (``None``).
+    A block holding an infinity or a NaN gets a NaN scale; such blocks do not enter the computed ``global_scale``.
+    """
+    _lib.require_cuda(x, global_scale)
+    assert block in _SCALE_DTYPE, "block is 16 or 32"
+    assert x.dim() in (2, 3), "x is [rows, cols] or [mats, rows, cols]"
+    rows, cols = x.shape[-2:]
+    mats = x.shape[0] if x.dim() == 3 else 1
+    assert cols > 0 and cols % block == 0, f"the row length must be a multiple of {block}"
+    assert x.stride(-1) == 1, "the elements of a row must be adjacent"
+    assert block == 16 or global_scale is None, "block 32 has no global scale"
+    check_global(global_scale, mats, block)
+    dev = x.device
+    _lib.require_device(dev, global_scale)
+    lead = x.shape[:-1]
+    with _lib.on_device(dev):
+        q = torch.empty(*lead, cols // 2, dtype=torch.uint8, device=dev)
+        scale = torch.empty(*lead, cols // block, dtype=_SCALE_DTYPE[block], device=dev)
+        own = block == 16 and global_scale is None
+        if own:
+            global_scale = (torch.empty if rows else torch.ones)(mats, dtype=torch.float32, device=dev)
+        if mats == 0 or rows == 0:
+            return q, scale, global_scale
+        lib = _lib.load()
+        ws, nbytes = None, 0
+        if own:
+            nbytes = lib.fr_fp4_quantize_workspace_bytes(mats, rows, cols)
+            ws = _lib.call_workspace(nbytes, dev, "fp4")
+        rc = lib.fr_fp4_quantize(_lib.ptr(x), _lib.dtype_code(x.dtype), mats, rows, cols,
+                                 x.stride(0) if x.dim() == 3 else 0, x.stride(-2) if rows > 1 else cols, block,
+                                 _lib.ptr(global_scale), 1 if own else 0, _lib.ptr(q), _lib.ptr(scale), _lib.ptr(ws),
+                                 nbytes, _lib.stream_ptr(dev))
+    _lib.check(rc, "fr_fp4_quantize")
+    return q, scale, global_scale
+
+
+def dequantize_fp4(q: torch.Tensor, scale: torch.Tensor, global_scale: torch.Tensor = None,
+                   dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The numbers that codes and scales stand for, rounded once to ``dtype`` (fp16, bf16 or fp32)."""
+    _lib.require_cuda(q, scale, global_scale)
+    assert q.dim() in (2, 3), "codes are [rows, cols/2] or [mats, rows, cols/2]"
+    block = block_of(q, scale)
+    rows, cols = q.shape[-2], q.shape[-1] * 2
+    mats = q.shape[0] if q.dim() == 3 else 1
+    check_global(global_scale, mats, block)
+    dev = q.device
+    _lib.require_device(dev, scale, global_scale)
+    code = _lib.dtype_code(dtype)
+    with _lib.on_device(dev):
+        out = torch.empty(*q.shape[:-1], cols, dtype=dtype, device=dev)
+        if out.numel() == 0:
+            return out
+        rc = _lib.load().fr_fp4_dequantize(_lib.ptr(q), _lib.ptr(scale), _lib.ptr(global_scale), mats, rows, cols, block,
+                                           code, _lib.ptr(out), _lib.stream_ptr(dev))
+    _lib.check(rc, "fr_fp4_dequantize")
+    return out
+
+
+__all__ = ["quantize_fp4", "dequantize_fp4"]

@@ -288,6 +288,46 @@ int fr_w4a16_gemm(const void* a, int64_t lda, const int32_t* qweight, const void
 int fr_w4a16_dequant(const int32_t* qweight, const void* scales, const int32_t* qzeros, int n, int k,
                      int groupsize, void* w, int64_t ldw, void* stream);
 
+/* Microscaled 4-bit floating point.  Codes are E2M1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two per byte, the
+ * even element in the low half; every block of consecutive elements of a row has a scale:
+ *   block 16: E4M3 and one fp32 scale per matrix, value = code * (scale * global);
+ *   block 32: E8M0 (2^(byte - 127), 0xFF = NaN),  value = code * scale.
+ * No counterpart in the reference (its only 4-bit format is the GPTQ integer one of fr_w4a16_gemm).
+ * fr_fp4_quantize: x[mats][rows][cols] (FR_F16 / FR_BF16 / FR_F32; pitches ld_mat, ld_row in elements, elements of a
+ *   row adjacent) -> q[mats][rows][cols / 2], scale[mats][rows][cols / block], dense.  block 16: with own_global != 0
+ *   global_scale[mats] is computed (largest finite-block magnitude / 2688, 1 for a matrix of zeros, at least 2^-110)
+ *   and written, else read; scale = e4m3(amax / (6 * global)), code = e2m1(x * (1 / (scale * global))).  block 32:
+ *   scale = 2^(floor(log2 amax) - 2), code = e2m1(x / scale) saturated at 6.  All roundings to nearest even, every
+ *   operation a single fp32 rounding.  A block that holds an infinity or a NaN gets a NaN scale and zero codes.
+ *   cols must be a multiple of block, mats <= 65535; workspace: fr_fp4_quantize_workspace_bytes, needed with
+ *   own_global only, no initial state.
+ * fr_fp4_dequantize: the numbers, rounded to `dtype`; global_scale may be NULL (1). */
+size_t fr_fp4_quantize_workspace_bytes(int64_t mats, int64_t rows, int64_t cols);
+int fr_fp4_quantize(const void* x, int dtype, int64_t mats, int64_t rows, int64_t cols, int64_t ld_mat, int64_t ld_row,
+                    int block, float* global_scale, int own_global, void* q, void* scale, void* workspace,
+                    size_t workspace_bytes, void* stream);
+int fr_fp4_dequantize(const void* q, const void* scale, const float* global_scale, int64_t mats, int64_t rows,
+                      int64_t cols, int block, int dtype, void* out, void* stream);
+
+/* The whole layer for at most FR_DECODE_MAX_TOKENS tokens in one cooperative launch: the contract of fr_moe_layer
+ * (routing ties to the lower expert id, softmax by the same recipe) with 16-bit or 4-bit expert weights.
+ * Stands in for fused_moe, fast_route/fast_route/layers/stable_route.py:10-102, for single-token generation.
+ *   block 0: w1[E,2I,H], w2[E,H,I] in `dtype`; the scale and global arguments are ignored;
+ *   block 16 / 32: w1 / w2 packed codes as fr_fp4_quantize writes them with mats = E (block scales w1_scale
+ *   [E,2I,H/block], w2_scale [E,H,I/block]; block 16: w1_global / w2_global fp32[E], NULL = 1).  The activations stay in
+ *   `dtype` and the expanded weights are exact, so nothing but the weights' own quantisation is lost.  Block 32 needs
+ *   FR_BF16 and block scales between 2^-60 and 2^33.
+ * x[M,H] dense; gate as in fr_route_fused; out[M,H] may alias x.  topk_weights_out / topk_ids_out: both or neither.
+ * E <= 256; H and I multiples of 8 (block 0) or 32.  The workspace (256-byte aligned) starts with the control words of
+ * the grid barrier: zero it once before its first use (see fr_align); one workspace serves one stream at a time. */
+#define FR_DECODE_MAX_TOKENS 16
+size_t fr_moe_decode_workspace_bytes(int64_t M, int H, int I, int E, int topk);
+int fr_moe_decode(const void* x, const void* gate, int64_t gate_stride_h, int64_t gate_stride_e, const void* w1,
+                  const void* w1_scale, const float* w1_global, const void* w2, const void* w2_scale,
+                  const float* w2_global, int dtype, int block, int64_t M, int H, int I, int E, int topk,
+                  int renormalize, void* out, float* topk_weights_out, int32_t* topk_ids_out, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

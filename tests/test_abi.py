@@ -102,3 +102,54 @@ def test_host_chunk_plan_covers_the_batch_exactly():
             assert max(b - a for a, b in plan) <= chunk + max(256, chunk // 4)
             if M <= chunk:
                 assert plan == [(0, M)]
+
+
+def test_few_token_layer_and_fp4_checks_reject_before_any_launch(lib):
+    null, p = ctypes.c_void_p(None), ctypes.c_void_p(1 << 20)        # p is never dereferenced: every call is refused
+
+    def decode(M=2, H=64, I=64, E=4, k=2, dtype=1, block=0, x=p, w1=p, s1=p, ws=p, nbytes=1 << 30, tw=null, ti=null):
+        return lib.fr_moe_decode(x, p, 1, H, w1, s1, null, p, p, null, dtype, block, M, H, I, E, k, 1, p, tw, ti, ws, nbytes,
+                                 null)
+    assert decode(k=5) == -1 and decode(k=0) == -1 and decode(M=-1) == -1 and decode(block=8) == -1
+    assert decode(x=null) == -1 and decode(w1=null) == -1 and decode(block=16, s1=null) == -1
+    assert decode(tw=p) == -1 and decode(ti=p) == -1
+    assert decode(M=17) == -2 and decode(E=257) == -2 and decode(dtype=2) == -2 and decode(dtype=0, block=32) == -2
+    assert decode(H=60) == -3 and decode(I=20) == -3 and decode(H=40, block=16) == -3
+    assert decode(w1=ctypes.c_void_p((1 << 20) + 8)) == -3 and decode(ws=ctypes.c_void_p((1 << 20) + 128)) == -3
+    assert decode(ws=null) == -4 and decode(nbytes=1000) == -4
+    assert decode(M=0) == 0
+    assert lib.fr_moe_decode_workspace_bytes(17, 64, 64, 4, 2) == 0
+    assert lib.fr_moe_decode_workspace_bytes(16, 4096, 14336, 8, 2) < 8 << 20
+
+    def quant(dtype=1, mats=1, rows=64, cols=1024, block=16, g=p, own=1, q=p, ws=null, nbytes=0):
+        return lib.fr_fp4_quantize(p, dtype, mats, rows, cols, 0, cols, block, g, own, q, p, ws, nbytes, null)
+    assert quant(block=8) == -1 and quant(cols=0) == -1 and quant(rows=-1) == -1 and quant(g=null) == -1
+    assert quant(dtype=3) == -2 and quant(cols=1032) == -2 and quant(mats=65536) == -2
+    assert quant(q=ctypes.c_void_p((1 << 20) + 4)) == -3
+    assert quant() == -4 and quant(ws=p, nbytes=4) == -4
+    assert quant(rows=0) == 0 and quant(mats=0) == 0
+    assert lib.fr_fp4_dequantize(p, p, null, 1, 4, 40, 16, 1, p, null) == -2
+    assert lib.fr_fp4_dequantize(p, p, null, 1, 4, 64, 16, 7, p, null) == -2
+    assert lib.fr_fp4_dequantize(p, p, null, 1, 4, 64, 16, 1, null, null) == -1
+    assert lib.fr_fp4_dequantize(p, p, null, 1, 4, 64, 16, 1, ctypes.c_void_p((1 << 20) + 8), null) == -3
+
+
+@pytest.mark.parametrize("block", [16, 32])
+def test_fp4_oracle_rounds_to_the_nearest_code(block):
+    """The oracle against a search over all codes: no code is closer to x / scale than the chosen one, ties are even."""
+    import numpy as np
+    from oracle import fp4
+    rng = np.random.default_rng(0)
+    x = rng.standard_normal((8, 64)).astype(np.float32)
+    x[0, :16] = [0, .25, .75, 1.25, 1.75, 2.5, 3.5, 5, 6, -.25, -.75, -1.25, -1.75, -2.5, -3.5, -5]
+    code, sb, glob = fp4.quantize(x, block)
+    s = fp4.e4m3(sb) if block == 16 else fp4.e8m0(sb)
+    unit = np.repeat(s * (glob if glob is not None else 1.0), block, -1)
+    r = np.minimum(np.abs(x / unit), 6.0)
+    best = np.abs(r[..., None] - fp4.E2M1[:8]).min(-1)
+    assert (np.abs(r - np.abs(fp4.E2M1[code])) <= best + 1e-6).all()
+    assert (np.signbit(fp4.E2M1[code]) == np.signbit(x)).all()
+    packed = (code[:, 0::2] | code[:, 1::2] << 4).astype(np.uint8)
+    assert np.array_equal(fp4.unpack(packed), code)
+    if block == 16:
+        assert fp4.e4m3(sb).max() == 448.0               # the largest block takes the largest scale
