@@ -8,17 +8,16 @@
 // * Work is split by weight ROWS, not by tiles: the (active experts * I) row pairs of w1 and the H rows of w2 are cut
 //   into equal contiguous ranges, so every CTA streams the same number of bytes whatever the sizes (16-row tiles left
 //   up to a quarter of the CTAs without a last tile).
-// * Each lane owns a FIFO in shared memory that it alone fills (16-byte cp.async) and drains, so the stream needs no
-//   barriers and runs on across row tiles, across experts and across the grid barrier: the first weights of w2 are in
-//   flight while the last activations are still being written.
+// * Each warp owns a FIFO in shared memory that it alone fills (cp.async, full 128-byte lines) and drains, so the
+//   stream needs no block barriers and runs on across row tiles, across experts and across the grid barrier: the first
+//   weights of w2 are in flight while the last activations are still being written.
 // * The products are mma.sync m16n8k16 with the TOKENS on the 16-row side: 8 weight rows by 16 tokens per instruction
 //   (a tcgen05 tile would be 128 weight rows, too coarse to split a layer of a few thousand rows over 296 CTAs, and
 //   its operand has to pass through shared memory and a barrier).  A lane's 16 bytes are 8 consecutive k of one row;
 //   the dot product does not care about the order of k, so both operands use the same permutation of k and no data is
 //   moved between lanes.
-// * 4-bit experts are expanded in registers: shifting a code's exponent and fraction into place gives the value times
-//   a power of two, one multiplication by the block scale gives the exact 16-bit weight (E2M1 * E4M3 has at most six
-//   significant bits), so the arithmetic is that of 16-bit weights.
+// * 4-bit experts are expanded in registers to the exact 16-bit weight (E2M1 * E4M3 has at most six significant bits),
+//   so the arithmetic is that of 16-bit weights.
 //
 // The eight warps of a CTA split K; their partial sums meet in shared memory in warp order, so results do not depend
 // on timing.  fp32 accumulation throughout; the activations between the two products are rounded to the 16-bit type.
@@ -32,9 +31,8 @@ constexpr int kDecTokens = FR_DECODE_MAX_TOKENS;   // 16: the row side of the MM
 constexpr int kDecMaxExperts = 256;
 constexpr int kDecWarps = 8;
 constexpr int kDecThreads = 32 * kDecWarps;
-constexpr int kDecStages = 4;
-constexpr int kDecStageBytes = 2048;               // per warp: four 16-byte chunks per lane
-constexpr int kDecPartStride = 20;                 // floats per weight row of a partial tile: conflict-free stores
+constexpr int kDecStages = 2;
+constexpr int kDecStageBytes = 4096;               // per warp: 32 chunks of 128 bytes of a weight row
 
 enum { WF_16BIT = 0, WF_NV4 = 1, WF_MX4 = 2 };
 
@@ -56,17 +54,22 @@ struct DecodeParams {
   uint16_t* act;                 // [active expert][M][I]
 };
 
+// HI: more than 8 tokens.  Then there is room for one buffer of partial sums only (two CTAs share an SM).
+template <bool HI>
 struct DecodeSmem {
+  static constexpr int kTokens = HI ? 16 : 8;
+  static constexpr int kStride = HI ? 20 : 12;      // floats per weight row of a partial tile: conflict-free stores
+  static constexpr int kBufs = HI ? 1 : 2;          // two buffers in turn: one barrier per tile instead of two
   uint8_t ring[kDecWarps][kDecStages][kDecStageBytes];
-  float part[kDecWarps][32 * kDecPartStride];
-  float weight[kDecMaxExperts][kDecTokens];   // routing weight by slot (position in `list`) and token
-  uint32_t mask[kDecMaxExperts];              // by expert: bit t = token t goes there
+  float part[kBufs][kDecWarps][32 * kStride];
+  float weight[kDecMaxExperts][kTokens];      // routing weight by slot (position in `list`) and token
+  uint32_t mask[kDecMaxExperts];              // by expert: bit t = token t goes there; upper half: its slot
   uint16_t list[kDecMaxExperts];              // active experts in ascending order
   uint32_t scan[kDecWarps];
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t size) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -88,23 +91,32 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Expansion of packed codes.  expand(): the pairs (j, j + 4), j = 0..3, of a word's eight codes as 16-bit numbers
-// times kUnit^-1; mult(): the factor for a block.  The fields of E2M1 (bias 1) placed in the low exponent bits and the
-// top fraction bit of the 16-bit format are the value times 2^(1 - bias), subnormal 0.5 included.
+// Expansion of a word of eight packed codes to 16-bit numbers: value * block scale / kUnit, exact.  fp16 has a conversion
+// instruction (half the issue slots of the shifts: 4-bit experts of a 1-token layer 104 -> 90 us); bf16 has none.
 template <bool BF16, int WF>
 struct Fp4Expand {
   // what is left to multiply the sums with: the factors below keep every intermediate inside the 16-bit format
-  static constexpr float kUnit = WF == WF_MX4 ? 4294967296.0f /* 2^32 */ : (BF16 ? 65536.0f : 128.0f);
-  static __device__ __forceinline__ uint32_t mult(uint32_t byte) {
+  static constexpr float kUnit = WF == WF_MX4 ? 4294967296.0f /* 2^32 */ : (BF16 ? 65536.0f : 1.0f);
+  // the factors of a lane's 32 codes: two blocks of 16 (m[0], m[1]) or one of 32
+  static __device__ __forceinline__ void mult(uint32_t scales, uint32_t (&m)[2]) {
     if constexpr (WF == WF_MX4) {
       // bf16 only: 2^(byte - 127) * 2^94.  Scales above 2^33 overflow to infinity; far below 2^-60 the products with
       // small activations leave the fp32 range.
-      const uint32_t e = byte + 94;
-      const uint32_t b = byte == 0xFFu ? 0x7FC0u : (e < 255u ? e << 7 : 0x7F80u);
-      return b | (b << 16);
+      const uint32_t e = scales + 94;
+      const uint32_t b = scales == 0xFFu ? 0x7FC0u : (e < 255u ? e << 7 : 0x7F80u);
+      m[0] = m[1] = b | (b << 16);
     } else {
-      const float s = __fmul_rn(e4m3_f32(byte), BF16 ? 1.298074214633706907e33f /* 2^110 */ : 128.0f);
-      return pack2<BF16>(s, s);     // exact: four significant bits
+      uint32_t h;   // both scales in fp16, exact, NaN included
+      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(scales)));
+      if constexpr (BF16) {
+        const float2 f = unpack2<false>(h);
+        const float a = __fmul_rn(f.x, 1.298074214633706907e33f /* 2^110 */), b = __fmul_rn(f.y, 1.298074214633706907e33f);
+        m[0] = pack2<true>(a, a);     // exact: four significant bits
+        m[1] = pack2<true>(b, b);
+      } else {
+        m[0] = __byte_perm(h, h, 0x1010);
+        m[1] = __byte_perm(h, h, 0x3232);
+      }
     }
   }
   static __device__ __forceinline__ uint32_t mul(uint32_t a, uint32_t m) {
@@ -114,18 +126,16 @@ struct Fp4Expand {
     return r;
   }
   static __device__ __forceinline__ void expand(uint32_t w, uint32_t m, uint32_t (&o)[4]) {
-    constexpr uint32_t S = 0x80008000u;
-    constexpr uint32_t F = BF16 ? 0x01C001C0u : 0x0E000E00u;
     if constexpr (BF16) {
+      // pairs (j, j + 4), as the fields of E2M1 (bias 1) in the low exponent bits and the top fraction bit of bf16:
+      // the value times 2^-126, subnormal 0.5 included
+      constexpr uint32_t S = 0x80008000u, F = 0x01C001C0u;
       o[0] = ((w << 12) & S) | ((w << 6) & F);
       o[1] = ((w << 8) & S) | ((w << 2) & F);
       o[2] = ((w << 4) & S) | ((w >> 2) & F);
       o[3] = (w & S) | ((w >> 6) & F);
     } else {
-      o[0] = ((w << 12) & S) | ((w << 9) & F);
-      o[1] = ((w << 8) & S) | ((w << 5) & F);
-      o[2] = ((w << 4) & S) | ((w << 1) & F);
-      o[3] = (w & S) | ((w >> 3) & F);
+      cvt8_f16(w, o);                 // pairs (2j, 2j + 1)
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] = mul(o[j], m);
@@ -133,16 +143,17 @@ struct Fp4Expand {
 };
 
 // One token row's operand for the 64 bytes of weights a quad holds: `p` points at the lane's first element.
-// 16-bit weights: 8 elements; 4-bit: 32 elements, reordered to the pairs (j, j + 4) that Fp4Expand makes.
-template <int WF>
+// 16-bit weights: 8 elements; 4-bit: 32 elements, for bf16 reordered to the pairs (j, j + 4) that Fp4Expand makes.  ANY
+// false: the row is known to be absent (tokens 8-15 of a batch of at most 8).
+template <bool BF16, int WF, bool ANY = true>
 __device__ __forceinline__ void load_tokens(const uint16_t* p, bool valid, bool coherent, uint32_t (&r)[WF == WF_16BIT ? 4 : 16]) {
   constexpr int NV = WF == WF_16BIT ? 1 : 4;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     uint4 u = make_uint4(0, 0, 0, 0);
-    if (valid) u = coherent ? __ldcg(reinterpret_cast<const uint4*>(p) + v) : __ldg(reinterpret_cast<const uint4*>(p) + v);
-    if constexpr (WF == WF_16BIT) {
-      r[0] = u.x, r[1] = u.y, r[2] = u.z, r[3] = u.w;
+    if (ANY && valid) u = coherent ? __ldcg(reinterpret_cast<const uint4*>(p) + v) : __ldg(reinterpret_cast<const uint4*>(p) + v);
+    if constexpr (WF == WF_16BIT || !BF16) {
+      r[4 * v] = u.x, r[4 * v + 1] = u.y, r[4 * v + 2] = u.z, r[4 * v + 3] = u.w;
     } else {
       r[4 * v] = __byte_perm(u.x, u.z, 0x5410);
       r[4 * v + 1] = __byte_perm(u.x, u.z, 0x7632);
@@ -163,13 +174,13 @@ __device__ __forceinline__ void chunk_mma(float (&acc)[4], const uint4& w, uint3
     mma_16816<BF16>(acc, a1, w.z, w.w);
   } else {
     using X = Fp4Expand<BF16, WF>;
-    const uint32_t m0 = X::mult(scales & 0xFFu);
-    const uint32_t m1 = WF == WF_NV4 ? X::mult(scales >> 8) : m0;   // a lane's 32 codes: two blocks of 16 or one of 32
+    uint32_t m[2];
+    X::mult(scales, m);
     const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t o[4];
-      X::expand(ww[i], i < 2 ? m0 : m1, o);
+      X::expand(ww[i], m[i >> 1], o);
       const uint32_t a0[4] = {lo[4 * i], hi[4 * i], lo[4 * i + 1], hi[4 * i + 1]};
       const uint32_t a1[4] = {lo[4 * i + 2], hi[4 * i + 2], lo[4 * i + 3], hi[4 * i + 3]};
       mma_16816<BF16>(acc, a0, o[0], o[1]);
@@ -178,13 +189,12 @@ __device__ __forceinline__ void chunk_mma(float (&acc)[4], const uint4& w, uint3
   }
 }
 
-// the scale bytes of the 16 bytes of codes at byte offset kb of a row
+// the scale bytes of a lane's 16 bytes of codes
 template <int WF>
-__device__ __forceinline__ uint32_t load_scales(const uint8_t* row, int kb, bool valid) {
-  if constexpr (WF == WF_16BIT) return 0;
+__device__ __forceinline__ uint32_t load_scales(const uint8_t* at, bool valid) {
   if (!valid) return 0;
-  if constexpr (WF == WF_NV4) return __ldg(reinterpret_cast<const uint16_t*>(row + (kb >> 3)));
-  return __ldg(row + (kb >> 4));
+  if constexpr (WF == WF_NV4) return __ldg(reinterpret_cast<const uint16_t*>(at));
+  return __ldg(at);
 }
 
 // ---- router: logits of all (token, expert) pairs, spread over the grid --------------------------------------
@@ -251,7 +261,8 @@ __device__ __forceinline__ uint32_t order_key(float v) {   // larger value, larg
 
 // Every CTA ranks all tokens: one warp per token, k rounds of arg-max (equal logits: lower expert id), softmax by the
 // fixed fp32 recipe of the routers.  `sel` / `val`: [kDecTokens][E] scratch.
-__device__ __forceinline__ void decode_rank(const DecodeParams& p, DecodeSmem& sm, uint16_t* sel, float* val) {
+template <bool HI>
+__device__ __forceinline__ void decode_rank(const DecodeParams& p, DecodeSmem<HI>& sm, uint16_t* sel, float* val) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int e = threadIdx.x; e < p.E; e += kDecThreads) sm.mask[e] = 0;
   __syncthreads();
@@ -331,17 +342,19 @@ __device__ __forceinline__ void decode_rank(const DecodeParams& p, DecodeSmem& s
   __syncthreads();
 }
 
-template <bool BF16, int WF>
+template <bool BF16, int WF, bool HI>
 __global__ void __launch_bounds__(kDecThreads, 2) moe_decode_kernel(const DecodeParams p) {
-  extern __shared__ __align__(16) uint8_t dec_smem[];
-  DecodeSmem& sm = *reinterpret_cast<DecodeSmem*>(dec_smem);
+  extern __shared__ __align__(128) uint8_t dec_smem[];
+  using Smem = DecodeSmem<HI>;
+  Smem& sm = *reinterpret_cast<Smem*>(dec_smem);
+  constexpr int PS = Smem::kStride;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
   const unsigned int G = gridDim.x;
 
-  decode_logits<BF16>(p, &sm.part[0][0]);
+  decode_logits<BF16>(p, &sm.part[0][0][0]);
   if (!grid_barrier(p.barrier, G)) return;
-  decode_rank(p, sm, reinterpret_cast<uint16_t*>(&sm.part[0][0]), reinterpret_cast<float*>(&sm.ring[0][0][0]));
+  decode_rank(p, sm, reinterpret_cast<uint16_t*>(&sm.part[0][0][0]), reinterpret_cast<float*>(&sm.ring[0][0][0]));
   int n_active = 0;
   for (int w = 0; w < kDecWarps; ++w) n_active += sm.scan[w];
 
@@ -357,80 +370,109 @@ __global__ void __launch_bounds__(kDecThreads, 2) moe_decode_kernel(const Decode
   const int row0 = static_cast<int>(static_cast<int64_t>(p.H) * blockIdx.x / G);
   const int row1 = static_cast<int>(static_cast<int64_t>(p.H) * (blockIdx.x + 1) / G);
 
-  // GEMM1: tiles of 16 pairs = four sub-tiles of 4 SiLU + 4 linear rows, 64 bytes of K per step, warp w takes steps
-  // w, w + 8, ...; GEMM2: tiles of 16 rows = two sub-tiles of 8 rows, 128 bytes of K per step, the steps of all active
-  // experts in one sequence dealt to the warps in turn.
-  const int nb1 = (rb1 + 63) / 64, nb2 = (rb2 + 127) / 128;
+  // A step is 128 bytes (a full line) of every row of a tile.  GEMM1: tiles of 16 pairs = four sub-tiles of 4 SiLU + 4
+  // linear rows, warp w takes steps w, w + 8, ...; GEMM2: tiles of 16 rows = two sub-tiles of 8, two steps at a time,
+  // the double steps of all active experts in one sequence dealt to the warps in turn.
+  const int nb1 = (rb1 + 127) / 128, nb2 = (rb2 + 255) / 256;
 
-  // ---- the loading end of the stream ----
-  int64_t ld_left = pair1 - pair0;     // pairs not yet fully requested
+  // ---- the loading end of the stream: one segment = one row tile of GEMM1, or one (row tile, expert) of GEMM2 ----
+  // Warp w's steps of a segment are b0, b0 + 8, ...; ld_rem counts those still to be requested.  Eight lanes copy one
+  // row's 128 bytes, four rows per instruction.  Rows past the tile are not copied (what the FIFO holds there ends up
+  // in sums nobody reads); k past the row's end is filled with zeros.
+  const int cr = lane >> 3, cc = lane & 7;
+  int64_t ld_left = pair1 - pair0;     // GEMM1 pairs from the next segment on
   int ld_a = static_cast<int>(pair0 / p.I), ld_j = static_cast<int>(pair0 - static_cast<int64_t>(ld_a) * p.I);
-  int ld_b = warp;
-  bool ld_first = warp < nb1 && ld_left > 0;
-  int ld_row = row0, ld_slot = 0;
-  auto settle2 = [&](int& slot, int& b) {
-    while (slot < n_active && b >= nb2) b -= nb2, ++slot;
-  };
-  int ld_b2 = warp;
-  settle2(ld_slot, ld_b2);
-  int ld_stage = 0;
-  const uint32_t ring = smem_u32(&sm.ring[warp][0][0]) + lane * 16;
+  int ld_row = row0, ld_slot = 0, ld_b2 = warp;
+  int ld_rem = 0, ld_k = 0, ld_rows = 0;
+  bool ld_second = false;
+  const uint8_t* ld_src = p.w1;
+  // chunk c of row r sits at position c ^ 4 * (r & 1) of the row: the reads below then touch every bank once
+  const uint32_t ring = smem_u32(&sm.ring[warp][0][0]) + cr * 128 + ((cc ^ ((cr & 1) << 2)) << 4);
+  uint32_t ld_at = 0, at_off = 0;
+  constexpr uint32_t RING = kDecStages * kDecStageBytes;
+  const int64_t lin1 = static_cast<int64_t>(p.I) * rb1;     // from a SiLU row to its linear row
   auto issue = [&]() {
-    const uint32_t dst = ring + ld_stage * kDecStageBytes;
-    if (ld_first) {
-      const int cnt = static_cast<int>(min(static_cast<int64_t>(min(16, p.I - ld_j)), ld_left));
-      const int kb = ld_b * 64 + t4 * 16;
-      const int64_t row = static_cast<int64_t>(sm.list[ld_a]) * 2 * p.I + (g < 4 ? 0 : p.I) + ld_j + (g & 3);
-      const uint8_t* src = p.w1 + row * rb1 + kb;
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const bool ok = 4 * s + (g & 3) < cnt && kb < rb1;
-        cp_async16(dst + s * 512, ok ? src + static_cast<int64_t>(4 * s) * rb1 : p.w1, ok);
-      }
-      ld_b += kDecWarps;
-      if (ld_b >= nb1) {
-        ld_b = warp;
+    while (ld_rem == 0) {              // next segment; the loop is for segments that have no step for this warp
+      if (ld_left > 0) {
+        const int cnt = static_cast<int>(min(static_cast<int64_t>(min(16, p.I - ld_j)), ld_left));
+        const int64_t row = static_cast<int64_t>(sm.list[ld_a]) * 2 * p.I + ld_j + cr;
+        ld_k = warp * 128 + cc * 16;
+        ld_src = p.w1 + row * rb1 + ld_k;
+        ld_rows = cnt - cr;
+        ld_rem = warp < nb1 ? (nb1 - warp + kDecWarps - 1) / kDecWarps : 0;
         ld_left -= cnt;
         ld_j += cnt;
         if (ld_j == p.I) ld_j = 0, ++ld_a;
-        ld_first = ld_left > 0;
-      }
-    } else if (ld_row < row1 && ld_slot < n_active) {
-      const int64_t row = static_cast<int64_t>(sm.list[ld_slot]) * p.H + ld_row + g;
-      const uint8_t* src = p.w2 + row * rb2;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          const int kb = ld_b2 * 128 + st * 64 + t4 * 16;
-          const bool ok = ld_row + 8 * s + g < row1 && kb < rb2;
-          cp_async16(dst + (s * 2 + st) * 512, ok ? src + static_cast<int64_t>(8 * s) * rb2 + kb : p.w2, ok);
+      } else if (ld_row < row1) {
+        ld_second = true;
+        const int64_t row = static_cast<int64_t>(sm.list[ld_slot]) * p.H + ld_row + cr;
+        ld_k = ld_b2 * 256 + cc * 16;
+        ld_src = p.w2 + row * rb2 + ld_k;
+        ld_rows = row1 - ld_row - cr;
+        if (ld_b2 < nb2) ld_rem = (nb2 - ld_b2 + kDecWarps - 1) / kDecWarps;
+        ld_b2 += ld_rem * kDecWarps - nb2;
+        if (++ld_slot == n_active) {
+          ld_slot = 0;
+          ld_b2 = warp;
+          ld_row += 16;
         }
-      }
-      ld_b2 += kDecWarps;
-      settle2(ld_slot, ld_b2);
-      if (ld_slot >= n_active) {
-        ld_row += 16;
-        ld_slot = 0;
-        ld_b2 = warp;
-        settle2(ld_slot, ld_b2);
+      } else {
+        cp_async_commit();
+        return;
       }
     }
+    const uint32_t dst = ring + ld_at;
+    if (!ld_second) {
+      const uint32_t size = ld_k < rb1 ? 16u : 0u;
+      const uint8_t* src = ld_src;
+      const int64_t step = static_cast<int64_t>(4) * rb1;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        if (4 * s < ld_rows) {
+          cp_async16(dst + s * 1024, src, size);
+          cp_async16(dst + s * 1024 + 512, src + lin1, size);
+        }
+        src += step;
+      }
+      ld_k += kDecWarps * 128;
+      ld_src += kDecWarps * 128;
+    } else {
+      const uint32_t size0 = ld_k < rb2 ? 16u : 0u, size1 = ld_k + 128 < rb2 ? 16u : 0u;
+      const uint8_t* src = ld_src;
+      const int64_t step = static_cast<int64_t>(4) * rb2;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {        // half a sub-tile: 4 rows
+        if (4 * s < ld_rows) {
+          cp_async16(dst + s * 512, src, size0);
+          cp_async16(dst + s * 512 + 2048, src + 128, size1);
+        }
+        src += step;
+      }
+      ld_k += kDecWarps * 256;
+      ld_src += kDecWarps * 256;
+    }
+    --ld_rem;
     cp_async_commit();
-    ld_stage = ld_stage + 1 == kDecStages ? 0 : ld_stage + 1;
+    ld_at = (ld_at + kDecStageBytes) & (RING - 1);
   };
-  int stage = 0;
-  auto next_stage = [&]() {   // request one more, then wait for the oldest
-    issue();
+  // the reading end: lane (g, t4) takes chunk t4 + 4 * st of row g of a sub-tile
+  const uint8_t* fifo = &sm.ring[warp][0][0] + g * 128 + ((t4 ^ ((g & 1) << 2)) << 4);
+  auto next_stage = [&]() {
     cp_async_wait<kDecStages - 1>();
-    const uint8_t* at = &sm.ring[warp][stage][lane * 16];
-    stage = stage + 1 == kDecStages ? 0 : stage + 1;
+    __syncwarp();
+    const uint8_t* at = fifo + at_off;
+    at_off = (at_off + kDecStageBytes) & (RING - 1);
     return at;
   };
+  auto chunk = [&](const uint8_t* at, int st) {   // st: 0 or 1; the other half of a row is at ^ 64
+    return *reinterpret_cast<const uint4*>(st ? reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(at) ^ 64) : at);
+  };
 #pragma unroll
-  for (int s = 0; s < kDecStages - 1; ++s) issue();
+  for (int s = 0; s < kDecStages; ++s) issue();
 
   constexpr int TR = WF == WF_16BIT ? 4 : 16;
+  constexpr int SPB = WF == WF_NV4 ? 8 : 4;        // scale bytes per 64 bytes of codes
+  int buf = 0;                                     // partial-sum buffer of the current tile
   // ---- GEMM1 + SiLU ----
   {
     int64_t left = pair1 - pair0;
@@ -445,40 +487,64 @@ __global__ void __launch_bounds__(kDecThreads, 2) moe_decode_kernel(const Decode
       for (int s = 0; s < 4; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[s][i] = 0.0f;
-      const uint16_t* x_lo = p.x + static_cast<int64_t>(g) * p.H;
-      const uint8_t* srow = p.s1 + (static_cast<int64_t>(e) * 2 * p.I + (g < 4 ? 0 : p.I) + j0 + (g & 3)) * sb1;
+      int kb = warp * 128 + t4 * 16;
+      const uint16_t* xp = p.x + static_cast<int64_t>(g) * p.H + (warp * 8 + t4) * ELT;
+      const int64_t x_hi = static_cast<int64_t>(8) * p.H;
+      const uint8_t* sp = p.s1 + (static_cast<int64_t>(e) * 2 * p.I + (g < 4 ? 0 : p.I) + j0 + (g & 3)) * sb1 +
+                          (WF == WF_NV4 ? kb >> 3 : kb >> 4);
+      const int64_t sb4 = static_cast<int64_t>(4) * sb1;
       for (int b = warp; b < nb1; b += kDecWarps) {
-        const int kb = b * 64 + t4 * 16, k = (b * 4 + t4) * ELT;
-        uint32_t lo[TR], hi[TR];
-        load_tokens<WF>(x_lo + k, use_lo && kb < rb1, false, lo);
-        load_tokens<WF>(x_lo + static_cast<int64_t>(8) * p.H + k, use_hi && kb < rb1, false, hi);
-        uint32_t sc[4];
+        uint32_t lo[2][TR], hi[2][TR];
+        const uint8_t* at = nullptr;
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-          sc[s] = load_scales<WF>(srow + static_cast<int64_t>(4 * s) * sb1, kb, 4 * s + (g & 3) < cnt && kb < rb1);
-        const uint8_t* at = next_stage();
+        for (int st = 0; st < 2; ++st) {
+          const bool in = kb + st * 64 < rb1;
+          load_tokens<BF16, WF>(xp + st * 4 * ELT, use_lo && in, false, lo[st]);
+          load_tokens<BF16, WF, HI>(xp + st * 4 * ELT + x_hi, use_hi && in, false, hi[st]);
+          uint32_t sc[4] = {0, 0, 0, 0};
+          if constexpr (WF != WF_16BIT) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-          chunk_mma<BF16, WF>(acc[s], *reinterpret_cast<const uint4*>(at + s * 512), sc[s], lo, hi);
+            for (int s = 0; s < 4; ++s) sc[s] = load_scales<WF>(sp + s * sb4 + st * SPB, 4 * s + (g & 3) < cnt && in);
+          }
+          if (WF == WF_16BIT ? st == 1 : st == 0) at = next_stage();
+          if constexpr (WF != WF_16BIT) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+              chunk_mma<BF16, WF>(acc[s], chunk(at + s * 1024, st), sc[s], lo[st], hi[st]);
+          }
+        }
+        if constexpr (WF == WF_16BIT) {
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int st = 0; st < 2; ++st) chunk_mma<BF16, WF>(acc[s], chunk(at + s * 1024, st), 0, lo[st], hi[st]);
+        }
+        __syncwarp();
+        issue();
+        kb += kDecWarps * 128;
+        xp += kDecWarps * 8 * ELT;
+        sp += kDecWarps * 2 * SPB;
       }
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        float* o = sm.part[warp] + (8 * s + 2 * t4) * kDecPartStride + g;
+        float* o = sm.part[buf][warp] + (8 * s + 2 * t4) * PS + g;
         o[0] = acc[s][0];
-        o[kDecPartStride] = acc[s][1];
-        o[8] = acc[s][2];
-        o[kDecPartStride + 8] = acc[s][3];
+        o[PS] = acc[s][1];
+        if constexpr (HI) {
+          o[8] = acc[s][2];
+          o[PS + 8] = acc[s][3];
+        }
       }
       __syncthreads();
       {
-        const int j = threadIdx.x & 15, t = threadIdx.x >> 4;
+        const int j = threadIdx.x & 15, t = threadIdx.x >> 4;   // t >= M: the mask has no such bit
         if (j < cnt && ((mask >> t) & 1u)) {
-          const int r = (8 * (j >> 2) + (j & 3)) * kDecPartStride + t;
+          const int r = (8 * (j >> 2) + (j & 3)) * PS + t;
           float hg = 0.0f, hu = 0.0f;
 #pragma unroll
           for (int w = 0; w < kDecWarps; ++w) {
-            hg += sm.part[w][r];
-            hu += sm.part[w][r + 4 * kDecPartStride];
+            hg += sm.part[buf][w][r];
+            hu += sm.part[buf][w][r + 4 * PS];
           }
           if constexpr (WF != WF_16BIT) {
             const float f = (p.g1 ? __ldg(p.g1 + e) : 1.0f) * Fp4Expand<BF16, WF>::kUnit;
@@ -489,7 +555,8 @@ __global__ void __launch_bounds__(kDecThreads, 2) moe_decode_kernel(const Decode
           p.act[(static_cast<int64_t>(a) * p.M + t) * p.I + j0 + j] = static_cast<uint16_t>(v);
         }
       }
-      __syncthreads();
+      if constexpr (Smem::kBufs == 2) buf ^= 1;
+      else __syncthreads();
       left -= cnt;
       j0 += cnt;
       if (j0 == p.I) j0 = 0, ++a;
@@ -506,8 +573,6 @@ __global__ void __launch_bounds__(kDecThreads, 2) moe_decode_kernel(const Decode
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int i = 0; i < 4; ++i) tot[s][i] = acc[s][i] = 0.0f;
-    int slot = 0, b = warp;
-    settle2(slot, b);
     // An expert's sum enters a token's total only where the token is routed to it: an infinity or NaN in its weights
     // must not reach the other tokens through a product with zero.
     auto fold = [&](int from) {
@@ -515,7 +580,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) moe_decode_kernel(const Decode
       const uint32_t mask = sm.mask[e];
       float f = 1.0f;
       if constexpr (WF != WF_16BIT) f = (p.g2 ? __ldg(p.g2 + e) : 1.0f) * Fp4Expand<BF16, WF>::kUnit;
-      const float w_lo = sm.weight[from][g] * f, w_hi = sm.weight[from][g + 8] * f;
+      const float w_lo = sm.weight[from][g] * f, w_hi = HI ? sm.weight[from][(g + 8) % Smem::kTokens] * f : 0.0f;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
 #pragma unroll
@@ -525,40 +590,70 @@ __global__ void __launch_bounds__(kDecThreads, 2) moe_decode_kernel(const Decode
         }
       }
     };
-    while (slot < n_active) {
-      const int e = sm.list[slot];
-      const uint32_t mask = sm.mask[e];
-      const bool use_lo = (mask >> g) & 1u, use_hi = (mask >> (g + 8)) & 1u;
-      const uint16_t* a_lo = p.act + (static_cast<int64_t>(slot) * p.M + g) * p.I;
-      const uint8_t* srow = p.s2 + (static_cast<int64_t>(e) * p.H + r0 + g) * sb2;
-      uint32_t lo[2][TR], hi[2][TR], sc[2][2];
+    int b = warp;
+    for (int slot = 0; slot < n_active; ++slot) {
+      if (b < nb2) {
+        const int e = sm.list[slot];
+        const uint32_t mask = sm.mask[e];
+        const bool use_lo = (mask >> g) & 1u, use_hi = (mask >> (g + 8)) & 1u;
+        int kb = b * 256 + t4 * 16;
+        const uint16_t* ap = p.act + (static_cast<int64_t>(slot) * p.M + g) * p.I + (b * 16 + t4) * ELT;
+        const int64_t a_hi = static_cast<int64_t>(8) * p.I;
+        const uint8_t* sp = p.s2 + (static_cast<int64_t>(e) * p.H + r0 + g) * sb2 + (WF == WF_NV4 ? kb >> 3 : kb >> 4);
+        const int64_t sb8 = static_cast<int64_t>(8) * sb2;
+        for (; b < nb2; b += kDecWarps) {
+          const uint8_t* at = nullptr;
+          if constexpr (WF == WF_16BIT) {
+            uint32_t lo[4][TR], hi[4][TR];
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const int kb = b * 128 + st * 64 + t4 * 16, k = (b * 8 + st * 4 + t4) * ELT;
-        load_tokens<WF>(a_lo + k, use_lo && kb < rb2, true, lo[st]);
-        load_tokens<WF>(a_lo + static_cast<int64_t>(8) * p.I + k, use_hi && kb < rb2, true, hi[st]);
+            for (int st = 0; st < 4; ++st) {
+              const bool in = kb + st * 64 < rb2;
+              load_tokens<BF16, WF>(ap + st * 4 * ELT, use_lo && in, true, lo[st]);
+              load_tokens<BF16, WF, HI>(ap + st * 4 * ELT + a_hi, use_hi && in, true, hi[st]);
+            }
+            at = next_stage();
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-          sc[s][st] = load_scales<WF>(srow + static_cast<int64_t>(8 * s) * sb2, kb, r0 + 8 * s + g < row1 && kb < rb2);
+            for (int s = 0; s < 2; ++s)
+              if (r0 + 8 * s < row1) {
+#pragma unroll
+                for (int st = 0; st < 4; ++st)
+                  chunk_mma<BF16, WF>(acc[s], chunk(at + s * 1024 + (st >> 1) * 2048, st & 1), 0, lo[st], hi[st]);
+              }
+          } else {
+#pragma unroll
+            for (int st = 0; st < 4; ++st) {
+              const bool in = kb + st * 64 < rb2;
+              uint32_t lo[TR], hi[TR], sc[2];
+              load_tokens<BF16, WF>(ap + st * 4 * ELT, use_lo && in, true, lo);
+              load_tokens<BF16, WF, HI>(ap + st * 4 * ELT + a_hi, use_hi && in, true, hi);
+#pragma unroll
+              for (int s = 0; s < 2; ++s) sc[s] = load_scales<WF>(sp + s * sb8 + st * SPB, r0 + 8 * s + g < row1 && in);
+              if (st == 0) at = next_stage();
+#pragma unroll
+              for (int s = 0; s < 2; ++s)
+                if (r0 + 8 * s < row1)
+                  chunk_mma<BF16, WF>(acc[s], chunk(at + s * 1024 + (st >> 1) * 2048, st & 1), sc[s], lo, hi);
+            }
+          }
+          __syncwarp();
+          issue();
+          kb += kDecWarps * 256;
+          ap += kDecWarps * 16 * ELT;
+          sp += kDecWarps * 4 * SPB;
+        }
+        fold(slot);
       }
-      const uint8_t* at = next_stage();
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int st = 0; st < 2; ++st)
-          chunk_mma<BF16, WF>(acc[s], *reinterpret_cast<const uint4*>(at + (s * 2 + st) * 512), sc[s][st], lo[st], hi[st]);
-      const int was = slot;
-      b += kDecWarps;
-      settle2(slot, b);
-      if (slot != was) fold(was);
+      b -= nb2;
     }
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      float* o = sm.part[warp] + (8 * s + 2 * t4) * kDecPartStride + g;
+      float* o = sm.part[buf][warp] + (8 * s + 2 * t4) * PS + g;
       o[0] = tot[s][0];
-      o[kDecPartStride] = tot[s][1];
-      o[8] = tot[s][2];
-      o[kDecPartStride + 8] = tot[s][3];
+      o[PS] = tot[s][1];
+      if constexpr (HI) {
+        o[8] = tot[s][2];
+        o[PS + 8] = tot[s][3];
+      }
     }
     __syncthreads();
     {
@@ -566,11 +661,12 @@ __global__ void __launch_bounds__(kDecThreads, 2) moe_decode_kernel(const Decode
       if (t < p.M && r0 + r < row1) {
         float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kDecWarps; ++w) v += sm.part[w][r * kDecPartStride + t];
+        for (int w = 0; w < kDecWarps; ++w) v += sm.part[buf][w][r * PS + t];
         p.out[static_cast<int64_t>(t) * p.H + r0 + r] = static_cast<uint16_t>(pack2<BF16>(v, 0.0f));
       }
     }
-    __syncthreads();
+    if constexpr (Smem::kBufs == 2) buf ^= 1;
+    else __syncthreads();
   }
   cp_async_wait<0>();
 }
@@ -594,10 +690,11 @@ size_t moe_decode_workspace(int64_t M, int I, int E, int topk) {
   return decode_ws(M, I, E, topk).total;
 }
 
-template <bool BF16, int WF>
-static int launch_decode(const DecodeParams& p, cudaStream_t st) {
-  auto kern = moe_decode_kernel<BF16, WF>;
-  constexpr int smem = sizeof(DecodeSmem);
+// HI: more than 8 tokens, the second half of the MMA's row side is used
+template <bool BF16, int WF, bool HI>
+static int launch_decode_rows(const DecodeParams& p, cudaStream_t st) {
+  auto kern = moe_decode_kernel<BF16, WF, HI>;
+  constexpr int smem = sizeof(DecodeSmem<HI>);
   // resident CTAs of the device, looked up once (0 = not yet)
   constexpr int kMaxDevices = 64;
   static std::atomic<int> grids[kMaxDevices];
@@ -628,6 +725,11 @@ static int launch_decode(const DecodeParams& p, cudaStream_t st) {
   cfg.numAttrs = 1;
   FR_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, q));
   return FR_OK;
+}
+
+template <bool BF16, int WF>
+static int launch_decode(const DecodeParams& p, cudaStream_t st) {
+  return p.M > 8 ? launch_decode_rows<BF16, WF, true>(p, st) : launch_decode_rows<BF16, WF, false>(p, st);
 }
 
 int moe_decode_dispatch(const void* x, const void* gate, int64_t gsh, int64_t gse, const void* w1, const void* s1,
