@@ -61,6 +61,7 @@ SIGNATURES = {
     "fr_fp4_quantize_workspace_bytes": (_Z, [_L, _L, _L]),
     "fr_fp4_quantize": (_I, [_P, _I, _L, _L, _L, _L, _L, _I, _P, _I, _P, _P, _P, _Z, _P]),
     "fr_fp4_dequantize": (_I, [_P, _P, _P, _L, _L, _L, _I, _I, _P, _P]),
+    "fr_fp4_gemm": (_I, [_P, _P, _P, _P, _P, _P, _I, _L, _L, _L, _I, _P, _L, _P]),
     "fr_moe_decode_workspace_bytes": (_Z, [_L, _I, _I, _I, _I]),
     "fr_moe_decode": (_I, [_P, _P, _L, _L, _P, _P, _P, _P, _P, _P, _I, _I, _L, _I, _I, _I, _I, _I, _P, _P, _P, _P, _Z, _P]),
 }

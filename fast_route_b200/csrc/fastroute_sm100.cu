@@ -8,4 +8,5 @@
 #include "fr_ep.cu"
 #include "fr_fp4.cu"
 #include "fr_decode.cu"
+#include "fr_fp4_gemm.cu"
 #include "fr_api.cu"

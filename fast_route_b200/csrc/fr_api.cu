@@ -1483,6 +1483,13 @@ int fr_fp4_dequantize(const void* q, const void* scale, const float* global_scal
                                      static_cast<cudaStream_t>(stream));
 }
 
+int fr_fp4_gemm(const void* a_q, const void* a_scale, const float* a_global, const void* b_q, const void* b_scale,
+                const float* b_global, int block, int64_t m, int64_t n, int64_t k, int dtype, void* c, int64_t ldc,
+                void* stream) {
+  return fr::fp4_gemm_dispatch(a_q, a_scale, a_global, b_q, b_scale, b_global, block, m, n, k, dtype, c, ldc,
+                               static_cast<cudaStream_t>(stream));
+}
+
 size_t fr_moe_decode_workspace_bytes(int64_t M, int H, int I, int E, int topk) {
   return H > 0 ? fr::moe_decode_workspace(M, I, E, topk) : 0;
 }

@@ -96,4 +96,38 @@ def dequantize_fp4(q: torch.Tensor, scale: torch.Tensor, global_scale: torch.Ten
     return out
 
 
-__all__ = ["quantize_fp4", "dequantize_fp4"]
+def matmul_fp4(a_q: torch.Tensor, a_scale: torch.Tensor, b_q: torch.Tensor, b_scale: torch.Tensor,
+               a_global: torch.Tensor = None, b_global: torch.Tensor = None, dtype: torch.dtype = torch.bfloat16,
+               out: torch.Tensor = None) -> torch.Tensor:
+    """``c[m,n] = a[m,k] . b[n,k]^T`` of two quantised matrices of the same block size (``k`` a multiple of 32) on the
+    block-scaled tensor-core instructions, fp32 accumulation, rounded once to ``dtype`` (fp16 or bf16).  ``out`` may have
+    any row pitch."""
+    _lib.require_cuda(a_q, a_scale, b_q, b_scale, a_global, b_global, out)
+    assert a_q.dim() == 2 and b_q.dim() == 2, "codes are [rows, k/2]"
+    block = block_of(a_q, a_scale, "a_scale")
+    assert block_of(b_q, b_scale, "b_scale") == block, "both matrices take the same block size"
+    m, n, k = a_q.shape[0], b_q.shape[0], a_q.shape[1] * 2
+    assert b_q.shape[1] * 2 == k, "Incompatible dimensions"
+    assert k > 0 and k % 32 == 0, "k must be a multiple of 32"
+    check_global(a_global, 1, block, "a_global")
+    check_global(b_global, 1, block, "b_global")
+    dev = a_q.device
+    _lib.require_device(dev, a_scale, b_q, b_scale, a_global, b_global, out)
+    if out is not None:
+        assert out.shape == (m, n) and out.dtype in (torch.float16, torch.bfloat16), "out is [m, n] in fp16 or bf16"
+        assert out.stride(1) == 1 or n == 1, "the elements of a row of out must be adjacent"
+        assert m <= 1 or out.stride(0) >= n, "rows of out must not overlap"
+    with _lib.on_device(dev):
+        if out is None:
+            assert dtype in (torch.float16, torch.bfloat16), f"unsupported dtype {dtype}"
+            out = torch.empty(m, n, dtype=dtype, device=dev)
+        if m == 0 or n == 0:
+            return out
+        rc = _lib.load().fr_fp4_gemm(_lib.ptr(a_q), _lib.ptr(a_scale), _lib.ptr(a_global), _lib.ptr(b_q), _lib.ptr(b_scale),
+                                     _lib.ptr(b_global), block, m, n, k, _lib.dtype_code(out.dtype), _lib.ptr(out),
+                                     out.stride(0) if m > 1 else n, _lib.stream_ptr(dev))
+    _lib.check(rc, "fr_fp4_gemm")
+    return out
+
+
+__all__ = ["quantize_fp4", "dequantize_fp4", "matmul_fp4"]

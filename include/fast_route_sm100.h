@@ -309,6 +309,15 @@ int fr_fp4_quantize(const void* x, int dtype, int64_t mats, int64_t rows, int64_
 int fr_fp4_dequantize(const void* q, const void* scale, const float* global_scale, int64_t mats, int64_t rows,
                       int64_t cols, int block, int dtype, void* out, void* stream);
 
+/* Product of two such matrices, c[m,n] = a_global * b_global * sum_k a[m,k] b[n,k], on the block-scaled tensor-core
+ * instructions with fp32 accumulation; c in FR_F16 / FR_BF16 (row pitch ldc), rounded once.  a and b are dense rows as
+ * fr_fp4_quantize writes them (mats = 1), both with the same block size; the global scales are one fp32 each on the
+ * device, NULL = 1.  k must be a multiple of 32, the codes 16-byte aligned.  A row whose scales hold a NaN gives NaN in
+ * its row (column) of c only. */
+int fr_fp4_gemm(const void* a_q, const void* a_scale, const float* a_global, const void* b_q, const void* b_scale,
+                const float* b_global, int block, int64_t m, int64_t n, int64_t k, int dtype, void* c, int64_t ldc,
+                void* stream);
+
 /* The whole layer for at most FR_DECODE_MAX_TOKENS tokens in one cooperative launch: the contract of fr_moe_layer
  * (routing ties to the lower expert id, softmax by the same recipe) with 16-bit or 4-bit expert weights.
  * Stands in for fused_moe, fast_route/fast_route/layers/stable_route.py:10-102, for single-token generation.

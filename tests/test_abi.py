@@ -153,3 +153,15 @@ def test_fp4_oracle_rounds_to_the_nearest_code(block):
     assert np.array_equal(fp4.unpack(packed), code)
     if block == 16:
         assert fp4.e4m3(sb).max() == 448.0               # the largest block takes the largest scale
+
+
+def test_fp4_product_checks_reject_before_any_launch(lib):
+    null, p = ctypes.c_void_p(None), ctypes.c_void_p(1 << 20)
+
+    def gemm(m=4, n=8, k=64, block=16, dtype=1, a=p, c=p, ldc=8):
+        return lib.fr_fp4_gemm(a, p, null, p, p, null, block, m, n, k, dtype, c, ldc, null)
+    assert gemm(m=-1) == -1 and gemm(k=0) == -1 and gemm(block=8) == -1 and gemm(ldc=7) == -1
+    assert gemm(a=null) == -1 and gemm(c=null) == -1
+    assert gemm(k=48) == -2 and gemm(dtype=2) == -2 and gemm(m=1 << 32) == -2
+    assert gemm(a=ctypes.c_void_p((1 << 20) + 8)) == -3
+    assert gemm(m=0) == 0 and gemm(n=0) == 0
