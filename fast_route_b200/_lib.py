@@ -61,7 +61,8 @@ SIGNATURES = {
     "fr_fp4_quantize_workspace_bytes": (_Z, [_L, _L, _L]),
     "fr_fp4_quantize": (_I, [_P, _I, _L, _L, _L, _L, _L, _I, _P, _I, _P, _P, _P, _Z, _P]),
     "fr_fp4_dequantize": (_I, [_P, _P, _P, _L, _L, _L, _I, _I, _P, _P]),
-    "fr_fp4_gemm": (_I, [_P, _P, _P, _P, _P, _P, _I, _L, _L, _L, _I, _P, _L, _P]),
+    "fr_fp4_gemm_workspace_bytes": (_Z, [_L, _L, _L, _I]),
+    "fr_fp4_gemm": (_I, [_P, _P, _P, _P, _P, _P, _I, _L, _L, _L, _I, _P, _L, _P, _Z, _P]),
     "fr_moe_decode_workspace_bytes": (_Z, [_L, _I, _I, _I, _I]),
     "fr_moe_decode": (_I, [_P, _P, _L, _L, _P, _P, _P, _P, _P, _P, _I, _I, _L, _I, _I, _I, _I, _I, _P, _P, _P, _P, _Z, _P]),
 }
@@ -98,11 +99,17 @@ def dtype_code(dt: torch.dtype) -> int:
 
 
 def ptr(t):
-    return None if t is None else c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
+
+
+# the handle of a device's current stream, without building a Stream object where torch offers that (2 us per call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def stream_ptr(device=None):
-    return c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    if _raw_stream is not None and device is not None and device.index is not None:
+        return _raw_stream(device.index)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def check(rc: int, what: str) -> None:
@@ -155,7 +162,7 @@ _workspaces: dict = {}
 def workspace(nbytes: int, device, tag: str = "layer") -> torch.Tensor:
     """A cached, 1024-byte aligned byte buffer per (device, stream, tag); grows on demand.
     New buffers are zero-filled once (the align stage keeps its grid-barrier words there)."""
-    key = (torch.device(device).index, torch.cuda.current_stream(device).cuda_stream, tag)
+    key = (torch.device(device).index, stream_ptr(device), tag)
     buf = _workspaces.get(key)
     if buf is None or buf.numel() < nbytes + 1024:
         buf = torch.zeros(int(nbytes) + 1024, dtype=torch.uint8, device=device)

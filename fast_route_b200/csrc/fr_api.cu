@@ -1483,11 +1483,15 @@ int fr_fp4_dequantize(const void* q, const void* scale, const float* global_scal
                                      static_cast<cudaStream_t>(stream));
 }
 
+size_t fr_fp4_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k, int block) {
+  return fr::fp4_gemm_workspace(m, n, k, block);
+}
+
 int fr_fp4_gemm(const void* a_q, const void* a_scale, const float* a_global, const void* b_q, const void* b_scale,
                 const float* b_global, int block, int64_t m, int64_t n, int64_t k, int dtype, void* c, int64_t ldc,
-                void* stream) {
-  return fr::fp4_gemm_dispatch(a_q, a_scale, a_global, b_q, b_scale, b_global, block, m, n, k, dtype, c, ldc,
-                               static_cast<cudaStream_t>(stream));
+                void* workspace, size_t workspace_bytes, void* stream) {
+  return fr::fp4_gemm_dispatch(a_q, a_scale, a_global, b_q, b_scale, b_global, block, m, n, k, dtype, c, ldc, workspace,
+                               workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 size_t fr_moe_decode_workspace_bytes(int64_t M, int H, int I, int E, int topk) {

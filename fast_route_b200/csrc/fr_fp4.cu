@@ -318,7 +318,7 @@ static int fp4_quantize_block(const Fp4QuantParams& p, int64_t mats, int64_t col
 }
 
 size_t fp4_quantize_workspace(int64_t mats, int64_t rows, int64_t cols) {
-  if (mats <= 0 || rows <= 0 || cols <= 0) return 0;
+  if (mats <= 0 || rows <= 0 || cols <= 0 || rows * cols <= kFp4SmallElems) return 0;
   return (static_cast<size_t>(mats) * fp4_parts(mats, rows, cols) * sizeof(float) + 255) & ~size_t(255);
 }
 
@@ -331,9 +331,10 @@ int fp4_quantize_dispatch(const void* x, int dtype, int64_t mats, int64_t rows, 
   if (dtype != FR_F16 && dtype != FR_BF16 && dtype != FR_F32) return FR_ERR_UNSUPPORTED;
   if (cols % block || mats > 65535 || cols > (int64_t(1) << 30)) return FR_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(q) & 7)) return FR_ERR_ALIGN;
-  if (block == 16 && own_global && rows * cols > kFp4SmallElems &&
-      (!workspace || workspace_bytes < fp4_quantize_workspace(mats, rows, cols)))
-    return FR_ERR_WORKSPACE;
+  if (block == 16 && own_global) {
+    const size_t need = fp4_quantize_workspace(mats, rows, cols);
+    if (need && (!workspace || workspace_bytes < need)) return FR_ERR_WORKSPACE;
+  }
   Fp4QuantParams p;
   p.x = x;
   p.ld_mat = ld_mat;

@@ -7,9 +7,13 @@
 //
 //   warp 0       TMA producer: 128 bytes (256 codes) of every row per stage, 128-byte swizzle
 //   warp 1       MMA issuer: copies the stage's scales from shared to tensor memory (tcgen05.cp), four MMAs of K = 64
-//   warps 2-5    scale loaders: the scales lie row by row in global memory; cp.async puts each 4-byte group where the
-//                hardware wants it (32 rows x 4 row groups x 4 bytes = one 512-byte block per 128 rows)
-//   warps 6-13   epilogue: each takes 32 lanes and half the columns
+//   epilogue     eight warps, each takes 32 lanes and half the columns
+//
+// The scales lie row by row in global memory; the hardware wants, for 128 rows, 512-byte blocks of 32 rows x 4 row
+// groups x 4 bytes.  For more than 128 tokens a small kernel lays them out that way in the workspace first (6 MB for
+// 8192 x 14336 x 4096) and the producer fetches 2 KB blocks; loading them row by row inside the product, with at most
+// four stages of look-ahead, took four times the MMAs' own time (684 us instead of 185).  Up to 128 tokens a second
+// launch would cost more than it saves: four loader warps put each 4-byte group in its place with cp.async.
 //
 // Every stage has its own columns in tensor memory for its scales, so a copy never overwrites scales that an MMA in
 // flight may still read: the stage is refilled only after its MMAs have completed.
@@ -21,12 +25,17 @@
 
 namespace fr {
 
-constexpr int FG_THREADS = 14 * 32;
 constexpr int FG_LANES = 128;
 constexpr int FG_KSTAGE = 256;          // codes of K per stage: 128 bytes of a row
 
 template <int BN, int BLOCK>
 struct FgCfg {
+  static constexpr bool LAID = BN == 256;                              // scales come laid out from the workspace
+  static constexpr int LOADERS = LAID ? 0 : 4;                         // warps that load scales
+  // threads that issue MMAs, each for its own share of the columns; with two, a third one issues the scale copies
+  static constexpr int ISSUERS = BN == 256 ? 2 : 1;
+  static constexpr int EPI0 = 1 + ISSUERS + (ISSUERS > 1 ? 1 : 0) + LOADERS;   // first epilogue warp
+  static constexpr int THREADS = 32 * (EPI0 + 8);
   static constexpr int STAGES = BN == 256 ? 4 : (BN == 128 ? 6 : 8);
   static constexpr int A_BYTES = FG_LANES * 128;
   static constexpr int B_BYTES = BN * 128;
@@ -41,13 +50,13 @@ struct FgCfg {
   static constexpr int SF_COLS = SFA_COLS * (1 + BGRP);
   static constexpr int TMEM_COLS = 512;
   static_assert(BN + STAGES * SF_COLS <= TMEM_COLS, "tensor memory");
-  static_assert(SMEM <= 227 * 1024, "shared memory");
+  static_assert(SMEM <= 227 * 1024 && FG_LANES * (BN + 4) * 4 <= PIPE_BYTES, "shared memory");
   static_assert(STAGE_BYTES % 1024 == 0, "swizzled tiles start on 1024-byte boundaries");
 };
 
 struct FgParams {
   int64_t rows_a, rows_b;        // lane rows, column rows
-  const uint8_t *sa, *sb;        // scales, row pitch `spitch` bytes
+  const uint8_t *sa, *sb;        // scales: rows of pitch `spitch` bytes, or laid out [128-row group][stage][block]
   int spitch;
   int kstages;                   // stages along K
   int split;                     // CTAs of a cluster that share a tile (1 = persistent CTAs, no cluster)
@@ -100,12 +109,40 @@ __device__ __forceinline__ uint32_t fp4_idesc(int n, uint32_t sf_id) {
          ((BLOCK == 32 ? 1u : 0u) << 23) | (static_cast<uint32_t>(FG_LANES >> 7) << 27) | (sf_id << 29);
 }
 
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, uint32_t size) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
 }
 
+// a stage's scale blocks to tensor memory: NB K steps of 4 columns for the lane side, then for the column side, whose
+// 128-row groups lie side by side within a step
+template <int BN, int BLOCK>
+__device__ __forceinline__ void fg_copy_scales(uint32_t tsf, uint32_t sf) {
+  using C = FgCfg<BN, BLOCK>;
+  constexpr int NB = C::SBLK / 512;
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    tc_cp_scales(tsf + 4 * j, scale_desc(sf + j * 512));
+#pragma unroll
+    for (int h = 0; h < C::BGRP; ++h)
+      tc_cp_scales(tsf + C::SFA_COLS + 4 * (j * C::BGRP + h), scale_desc(sf + C::SBLK * (1 + h) + j * 512));
+  }
+}
+
+// Where a partial sum waits: the index that runs along a row of c is innermost, so that four of them are read at once.
+// (Not swapped: the pitch of BN + 4 floats gives the 16-byte stores of eight lanes, one row each, all 32 banks.)
+template <int BN>
+__device__ __forceinline__ int fg_park(int swapped, int row, int col) {
+  return swapped ? col * FG_LANES + row : row * (BN + 4) + col;
+}
+
 template <int BN, int BLOCK, bool BF16>
-__global__ void __launch_bounds__(FG_THREADS, 1)
+__global__ void __launch_bounds__((FgCfg<BN, BLOCK>::THREADS), 1)
 fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const FgParams p) {
   using C = FgCfg<BN, BLOCK>;
   constexpr int S = C::STAGES;
@@ -113,7 +150,8 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::PIPE_BYTES);
   uint64_t* empty = full + S;
-  uint64_t* tfull = empty + S;
+  uint64_t* sfull = empty + S;            // scales of the stage are in tensor memory (two issuers)
+  uint64_t* tfull = sfull + S;
   uint64_t* tempty = tfull + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -121,10 +159,11 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(&full[s], 1 + 4);         // the TMA producer and the four loader warps
-      mbar_init(&empty[s], 1);
+      mbar_init(&full[s], 1 + C::LOADERS);   // the TMA producer and the loader warps
+      mbar_init(&empty[s], C::ISSUERS);
+      mbar_init(&sfull[s], 1);
     }
-    mbar_init(tfull, 1);
+    mbar_init(tfull, C::ISSUERS);
     mbar_init(tempty, 8);
     *abort_flag = 0;
     mbar_fence_init();
@@ -160,16 +199,28 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             break;
           }
           uint8_t* st = smem + ps.stage * C::STAGE_BYTES;
-          mbar_expect_tx(&full[ps.stage], C::A_BYTES + C::B_BYTES);
+          mbar_expect_tx(&full[ps.stage], C::A_BYTES + C::B_BYTES + (C::LAID ? C::SF_BYTES : 0));
           tma_load_2d(st, &tmA, &full[ps.stage], k * 128, ra);
           tma_load_2d(st + C::A_BYTES, &tmB, &full[ps.stage], k * 128, rbb);
+          if constexpr (C::LAID) {
+            uint8_t* sf = st + C::A_BYTES + C::B_BYTES;
+            const int64_t ga = static_cast<int64_t>(tile % p.tiles_a) * p.kstages + k;
+            bulk_load(sf, p.sa + ga * C::SBLK, C::SBLK, &full[ps.stage]);
+#pragma unroll
+            for (int h = 0; h < C::BGRP; ++h) {
+              const int64_t gb = (static_cast<int64_t>(tile / p.tiles_a) * C::BGRP + h) * p.kstages + k;
+              bulk_load(sf + C::SBLK * (1 + h), p.sb + gb * C::SBLK, C::SBLK, &full[ps.stage]);
+            }
+          }
           ps.advance_rt(S);
         }
       }
     }
-  } else if (warp == 1) {
-    // ------------------------------ MMA issuer --------------------------------
+  } else if (warp <= C::ISSUERS) {
+    // ------------------------------ MMA issuers -------------------------------
     if (lane == 0) {
+      constexpr int NI = BN / C::ISSUERS;        // columns of this issuer: its own accumulators
+      const int part = warp - 1;
       PipeState ps;
       uint32_t it = 0;
       bool ok = true;
@@ -177,29 +228,22 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         if (!wait_or_abort(tempty, (it & 1u) ^ 1, abort_flag, 0x701)) break;
         tc_fence_after();
         for (int k = k0; k < k1; ++k) {
-          if (!wait_or_abort(&full[ps.stage], ps.phase, abort_flag, 0x702)) {
+          if (!wait_or_abort(&full[ps.stage], ps.phase, abort_flag, 0x702) ||
+              (C::ISSUERS > 1 && !wait_or_abort(&sfull[ps.stage], ps.phase, abort_flag, 0x705))) {
             ok = false;
             break;
           }
           tc_fence_after();
           const uint32_t st = smem_u32(smem + ps.stage * C::STAGE_BYTES);
-          const uint32_t sf = st + C::A_BYTES + C::B_BYTES;
           const uint32_t tsf = tmem + BN + ps.stage * C::SF_COLS;
-          constexpr int NB = C::SBLK / 512;      // 512-byte scale blocks per 128 rows: 4 (block 16) or 2 (block 32)
-#pragma unroll
-          for (int j = 0; j < NB; ++j) {
-            tc_cp_scales(tsf + 4 * j, scale_desc(sf + j * 512));
-#pragma unroll
-            for (int h = 0; h < C::BGRP; ++h)    // the column side's groups of one K step lie side by side
-              tc_cp_scales(tsf + C::SFA_COLS + 4 * (j * C::BGRP + h), scale_desc(sf + C::SBLK * (1 + h) + j * 512));
-          }
-          const uint64_t ad = umma_desc_sw128(st), bd = umma_desc_sw128(st + C::A_BYTES);
+          if constexpr (C::ISSUERS == 1) fg_copy_scales<BN, BLOCK>(tsf, st + C::A_BYTES + C::B_BYTES);
+          const uint64_t ad = umma_desc_sw128(st), bd = umma_desc_sw128(st + C::A_BYTES + part * NI * 128);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int blk = BLOCK == 16 ? j : j >> 1;
             const uint32_t id = BLOCK == 16 ? 0u : static_cast<uint32_t>(j & 1) * 2u;
-            tc_mma_fp4<BLOCK>(tmem, ad + 2 * j, bd + 2 * j, fp4_idesc<BLOCK>(BN, id), tsf + 4 * blk,
-                              tsf + C::SFA_COLS + 4 * blk * C::BGRP, (k > k0 || j > 0) ? 1u : 0u);
+            tc_mma_fp4<BLOCK>(tmem + part * NI, ad + 2 * j, bd + 2 * j, fp4_idesc<BLOCK>(NI, id), tsf + 4 * blk,
+                              tsf + C::SFA_COLS + 4 * (blk * C::BGRP + part), (k > k0 || j > 0) ? 1u : 0u);
           }
           tc_commit(&empty[ps.stage]);
           ps.advance_rt(S);
@@ -207,7 +251,27 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         if (ok) tc_commit(tfull);
       }
     }
-  } else if (warp < 6) {
+  } else if (C::ISSUERS > 1 && warp == C::ISSUERS + 1) {
+    // ------------------------------ scale copies ------------------------------
+    if (lane == 0) {
+      PipeState ps;
+      bool ok = true;
+      for (int tile = first; tile < tiles && ok; tile += stride) {
+        for (int k = k0; k < k1; ++k) {
+          if (!wait_or_abort(&full[ps.stage], ps.phase, abort_flag, 0x706)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          fg_copy_scales<BN, BLOCK>(tmem + BN + ps.stage * C::SF_COLS,
+                                    smem_u32(smem + ps.stage * C::STAGE_BYTES) + C::A_BYTES + C::B_BYTES);
+          tc_commit(&sfull[ps.stage]);
+          ps.advance_rt(S);
+        }
+      }
+    }
+  } else if (warp < C::EPI0) {
+    if constexpr (!C::LAID) {
     // ------------------------------ scale loaders -----------------------------
     // Thread r copies the scales of lane row r and of column rows r (and 128 + r).  The copies of two stages are in
     // flight behind the one being handed over.
@@ -235,7 +299,9 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           cp_async4(dst + w * 512, n > 0 ? src + kb + 4 * w : base, static_cast<uint32_t>(n));
         } else {
           uint32_t v = 0;
-          for (int i = 0; i < n; ++i) v |= static_cast<uint32_t>(__ldg(src + kb + 4 * w + i)) << (8 * i);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (i < n) v |= static_cast<uint32_t>(__ldg(src + kb + 4 * w + i)) << (8 * i);
           asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + w * 512), "r"(v) : "memory");
         }
       }
@@ -263,9 +329,10 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     }
     cp_async_wait<0>();
     while (pending > 0) hand_over();
+    }
   } else {
     // ------------------------------ epilogue ----------------------------------
-    const int q = warp & 3, half = (warp - 6) >> 2;       // lanes 32q .. 32q+31, columns of this half
+    const int q = warp & 3, half = (warp - C::EPI0) >> 2;       // lanes 32q .. 32q+31, columns of this half
     constexpr int HC = BN / 2 < 16 ? 16 : BN / 2;
     const float alpha = (p.ga ? __ldg(p.ga) : 1.0f) * (p.gb ? __ldg(p.gb) : 1.0f);
     uint32_t it = 0;
@@ -278,15 +345,22 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       tc_fence_after();
       const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + half * HC;
       if (p.split > 1) {
-        // park the partial tile, columns outermost, in the pipeline's memory: every MMA of this CTA has completed
+        // park the partial tile in the pipeline's memory: every MMA of this CTA has completed
         float* part = reinterpret_cast<float*>(smem);
 #pragma unroll 1
         for (int c0 = 0; c0 < HC; c0 += 16) {
           uint32_t v[16];
           tmem_ld16(taddr + c0, v);
           tc_wait_ld();
+          if (p.swapped) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) part[(half * HC + c0 + i) * FG_LANES + q * 32 + lane] = __uint_as_float(v[i]);
+            for (int i = 0; i < 16; ++i) part[fg_park<BN>(1, q * 32 + lane, half * HC + c0 + i)] = __uint_as_float(v[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+              *reinterpret_cast<uint4*>(part + fg_park<BN>(0, q * 32 + lane, half * HC + c0 + i)) =
+                  make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          }
         }
         break;                                             // one tile per cluster
       }
@@ -335,24 +409,42 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     cluster.sync();
     const bool ok = *abort_flag == 0;
     const float alpha = (p.ga ? __ldg(p.ga) : 1.0f) * (p.gb ? __ldg(p.gb) : 1.0f);
-    const int c_lo = BN * rank / p.split, c_hi = BN * (rank + 1) / p.split;
+    // slices of the tile's columns; BN / split is a multiple of 4
+    const int cols = BN / p.split, c_lo = cols * rank;
     const int64_t ra0 = static_cast<int64_t>(first % p.tiles_a) * FG_LANES;
     const int64_t rb0 = static_cast<int64_t>(first / p.tiles_a) * BN;
     const float* parts[8];
 #pragma unroll
     for (int s = 0; s < 8; ++s) parts[s] = cluster.map_shared_rank(reinterpret_cast<float*>(smem), s < p.split ? s : 0);
-    for (int i = threadIdx.x; ok && i < (c_hi - c_lo) * FG_LANES; i += FG_THREADS) {
-      int cc, rr;
-      if (p.swapped) cc = c_lo + i / FG_LANES, rr = i % FG_LANES;          // stores run along the lane rows
-      else rr = i / (c_hi - c_lo), cc = c_lo + i % (c_hi - c_lo);          // stores run along the columns
-      if (ra0 + rr >= p.rows_a || rb0 + cc >= p.rows_b) continue;
-      float v = 0.0f;
+    const bool pairs4 = p.ldc % 4 == 0 && !(reinterpret_cast<uintptr_t>(p.c) & 7);
+#pragma unroll 2
+    for (int i = threadIdx.x; ok && i < cols * FG_LANES / 4; i += C::THREADS) {
+      int cc, rr;                                     // four neighbours along a row of c start here
+      if (p.swapped) cc = c_lo + i / (FG_LANES / 4), rr = i % (FG_LANES / 4) * 4;
+      else rr = i / (cols / 4), cc = c_lo + i % (cols / 4) * 4;
+      const int64_t row = p.swapped ? rb0 + cc : ra0 + rr, col = p.swapped ? ra0 + rr : rb0 + cc;
+      const int64_t rows = p.swapped ? p.rows_b : p.rows_a, width = p.swapped ? p.rows_a : p.rows_b;
+      if (row >= rows || col >= width) continue;
+      const int at = fg_park<BN>(p.swapped, rr, cc);
+      float4 f[8];
 #pragma unroll
       for (int s = 0; s < 8; ++s)
-        if (s < p.split) v += parts[s][cc * FG_LANES + rr];
-      const uint16_t r16 = static_cast<uint16_t>(pack2<BF16>(v * alpha, 0.0f));
-      if (p.swapped) p.c[(rb0 + cc) * p.ldc + ra0 + rr] = r16;
-      else p.c[(ra0 + rr) * p.ldc + rb0 + cc] = r16;
+        if (s < p.split) f[s] = *reinterpret_cast<const float4*>(parts[s] + at);
+      float4 v = f[0];
+#pragma unroll
+      for (int s = 1; s < 8; ++s)
+        if (s < p.split) v.x += f[s].x, v.y += f[s].y, v.z += f[s].z, v.w += f[s].w;
+      const uint32_t lo = pack2<BF16>(v.x * alpha, v.y * alpha), hi = pack2<BF16>(v.z * alpha, v.w * alpha);
+      uint16_t* o = p.c + row * p.ldc + col;
+      if (pairs4 && col + 4 <= width) {
+        *reinterpret_cast<uint2*>(o) = make_uint2(lo, hi);
+      } else {
+        const uint16_t e[4] = {static_cast<uint16_t>(lo), static_cast<uint16_t>(lo >> 16), static_cast<uint16_t>(hi),
+                               static_cast<uint16_t>(hi >> 16)};
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (col + u < width) o[u] = e[u];
+      }
     }
     cluster.sync();                                          // nobody leaves while its memory is being read
   }
@@ -364,6 +456,49 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   }
 }
 
+// Scales [rows][spitch] -> [128-row group][stage][block of 512 bytes], zeros past the rows and past K.  One CTA: 128 rows
+// and up to four stages (64 or 32 contiguous bytes of a row), turned in shared memory and written out whole.
+struct FgLayout {
+  const uint8_t *sa, *sb;
+  uint8_t *da, *db;
+  int64_t rows_a, rows_b;
+  int groups_a;          // blockIdx.x below this: the lane side
+  int spitch, kstages;
+};
+template <int BLOCK>
+__global__ void __launch_bounds__(128) fp4_scale_layout_kernel(const FgLayout p) {
+  constexpr int SB = FG_KSTAGE / BLOCK, W = SB / 4, NS = 4;
+  __shared__ uint32_t sm[NS][W * 128];
+  const bool lane_side = static_cast<int>(blockIdx.x) < p.groups_a;
+  const int group = lane_side ? blockIdx.x : blockIdx.x - p.groups_a;
+  const uint8_t* s = lane_side ? p.sa : p.sb;
+  const int64_t rows = lane_side ? p.rows_a : p.rows_b, row = static_cast<int64_t>(group) * 128 + threadIdx.x;
+  const int k0 = blockIdx.y * NS, ns = min(NS, p.kstages - k0);
+  const uint8_t* src = s + row * p.spitch + static_cast<int64_t>(k0) * SB;
+  const int left = row < rows ? min(ns * SB, p.spitch - k0 * SB) : 0;
+  const bool word = ((p.spitch | static_cast<int>(reinterpret_cast<uintptr_t>(s))) & 3) == 0;
+  uint32_t v[NS * W];
+#pragma unroll
+  for (int i = 0; i < NS * W; ++i) {
+    v[i] = 0;
+    if (word) {
+      if (4 * i < left) v[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
+    } else {
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        if (4 * i + b < left) v[i] |= static_cast<uint32_t>(__ldg(src + 4 * i + b)) << (8 * b);
+    }
+  }
+  const int spot = (threadIdx.x & 31) * 4 + (threadIdx.x >> 5);
+#pragma unroll
+  for (int i = 0; i < NS * W; ++i) sm[i / W][(i % W) * 128 + spot] = v[i];
+  __syncthreads();
+  uint4* dst = reinterpret_cast<uint4*>((lane_side ? p.da : p.db) +
+                                        (static_cast<int64_t>(group) * p.kstages + k0) * (W * 512));
+  const uint4* from = reinterpret_cast<const uint4*>(&sm[0][0]);
+  for (int i = threadIdx.x; i < ns * W * 32; i += 128) dst[i] = from[i];
+}
+
 template <int BN, int BLOCK, bool BF16>
 static int launch_fp4_gemm(const CUtensorMap& a, const CUtensorMap& b, const FgParams& p, int grid, cudaStream_t st) {
   auto kern = fp4_gemm_kernel<BN, BLOCK, BF16>;
@@ -371,7 +506,7 @@ static int launch_fp4_gemm(const CUtensorMap& a, const CUtensorMap& b, const FgP
   FR_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(FG_THREADS);
+  cfg.blockDim = dim3(FgCfg<BN, BLOCK>::THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -393,52 +528,101 @@ static int launch_fp4_bn(const CUtensorMap& a, const CUtensorMap& b, const FgPar
   return bf ? launch_fp4_gemm<BN, 32, true>(a, b, p, grid, st) : launch_fp4_gemm<BN, 32, false>(a, b, p, grid, st);
 }
 
+// how a product is cut: tokens (m) on the column side while they fit into one tile of at most 128 columns
+struct FgPlan {
+  bool swapped;
+  int bn, kstages, groups_a, groups_b, tiles_a, tiles_b;
+  size_t sblk, ws_a, ws_total;
+};
+static FgPlan fp4_plan(int64_t m, int64_t n, int64_t k, int block) {
+  FgPlan q;
+  q.swapped = m <= 128;
+  q.bn = q.swapped ? (m <= 32 ? 32 : 128) : 256;
+  const int64_t ra = q.swapped ? n : m, rb = q.swapped ? m : n;
+  q.kstages = static_cast<int>((k + FG_KSTAGE - 1) / FG_KSTAGE);
+  q.tiles_a = static_cast<int>((ra + FG_LANES - 1) / FG_LANES);
+  q.tiles_b = static_cast<int>((rb + q.bn - 1) / q.bn);
+  q.groups_a = q.tiles_a;
+  q.groups_b = q.tiles_b * (q.bn / 128);
+  q.sblk = block == 16 ? 2048 : 1024;
+  q.ws_a = static_cast<size_t>(q.groups_a) * q.kstages * q.sblk;
+  q.ws_total = q.swapped ? 0 : q.ws_a + static_cast<size_t>(q.groups_b) * q.kstages * q.sblk;
+  return q;
+}
+static bool fp4_gemm_sizes_ok(int64_t m, int64_t n, int64_t k) {
+  constexpr int64_t kMax = int64_t(1) << 30;
+  return k % 32 == 0 && k <= (int64_t(1) << 28) && m <= kMax && n <= kMax &&
+         ((m + 127) / 128) * ((n + 127) / 128) <= kMax;
+}
+
+size_t fp4_gemm_workspace(int64_t m, int64_t n, int64_t k, int block) {
+  if (m <= 0 || n <= 0 || k <= 0 || (block != 16 && block != 32) || !fp4_gemm_sizes_ok(m, n, k)) return 0;
+  return fp4_plan(m, n, k, block).ws_total;
+}
+
 int fp4_gemm_dispatch(const void* a_q, const void* a_scale, const float* a_global, const void* b_q, const void* b_scale,
                       const float* b_global, int block, int64_t m, int64_t n, int64_t k, int dtype, void* c, int64_t ldc,
-                      cudaStream_t st) {
+                      void* workspace, size_t workspace_bytes, cudaStream_t st) {
   if (m < 0 || n < 0 || k <= 0 || (block != 16 && block != 32) || ldc < n) return FR_ERR_ARG;
   if (dtype != FR_F16 && dtype != FR_BF16) return FR_ERR_UNSUPPORTED;
-  if (k % 32 || k > (int64_t(1) << 28) || m > (int64_t(1) << 31) - 256 || n > (int64_t(1) << 31) - 256)
-    return FR_ERR_UNSUPPORTED;
+  if (!fp4_gemm_sizes_ok(m, n, k)) return FR_ERR_UNSUPPORTED;
   if (m == 0 || n == 0) return FR_OK;
   if (!a_q || !a_scale || !b_q || !b_scale || !c) return FR_ERR_ARG;
   if (((reinterpret_cast<uintptr_t>(a_q) | reinterpret_cast<uintptr_t>(b_q)) & 15) || (reinterpret_cast<uintptr_t>(c) & 1))
     return FR_ERR_ALIGN;
-  // tokens (m) on the column side while they fit into one tile of at most 128 columns
-  const bool swapped = m <= 128;
-  const int bn = swapped ? (m <= 32 ? 32 : 128) : 256;
+  const FgPlan q = fp4_plan(m, n, k, block);
+  if (q.ws_total && (!workspace || workspace_bytes < q.ws_total)) return FR_ERR_WORKSPACE;
+  if (q.ws_total && (reinterpret_cast<uintptr_t>(workspace) & 15)) return FR_ERR_ALIGN;
   FgParams p;
-  p.rows_a = swapped ? n : m;
-  p.rows_b = swapped ? m : n;
-  p.sa = static_cast<const uint8_t*>(swapped ? b_scale : a_scale);
-  p.sb = static_cast<const uint8_t*>(swapped ? a_scale : b_scale);
+  p.rows_a = q.swapped ? n : m;
+  p.rows_b = q.swapped ? m : n;
+  p.sa = static_cast<const uint8_t*>(q.swapped ? b_scale : a_scale);
+  p.sb = static_cast<const uint8_t*>(q.swapped ? a_scale : b_scale);
   p.spitch = static_cast<int>(k / block);
-  p.kstages = static_cast<int>((k + FG_KSTAGE - 1) / FG_KSTAGE);
-  const int64_t ta = (p.rows_a + FG_LANES - 1) / FG_LANES, tb = (p.rows_b + bn - 1) / bn;
-  if (ta * tb > (int64_t(1) << 30)) return FR_ERR_UNSUPPORTED;
-  p.tiles_a = static_cast<int>(ta);
-  p.tiles_b = static_cast<int>(tb);
+  p.kstages = q.kstages;
+  p.tiles_a = q.tiles_a;
+  p.tiles_b = q.tiles_b;
   p.ga = a_global;
   p.gb = b_global;
   p.c = static_cast<uint16_t*>(c);
   p.ldc = ldc;
-  p.swapped = swapped;
-  p.vec = !swapped && ldc % 8 == 0 && !(reinterpret_cast<uintptr_t>(c) & 15);
+  p.swapped = q.swapped;
+  p.vec = !q.swapped && ldc % 8 == 0 && !(reinterpret_cast<uintptr_t>(c) & 15);
+  CUtensorMap ma, mb;
+  const uint64_t kb = static_cast<uint64_t>(k / 2);
+  int rc = make_tmap_2d(&ma, q.swapped ? b_q : a_q, p.rows_a, kb, kb, FG_LANES, 128, true, 1);
+  if (rc) return rc;
+  rc = make_tmap_2d(&mb, q.swapped ? a_q : b_q, p.rows_b, kb, kb, q.bn, 128, true, 1);
+  if (rc) return rc;
+  if (!q.swapped) {
+    FgLayout l;
+    l.sa = p.sa;
+    l.sb = p.sb;
+    l.da = static_cast<uint8_t*>(workspace);
+    l.db = l.da + q.ws_a;
+    l.rows_a = p.rows_a;
+    l.rows_b = p.rows_b;
+    l.groups_a = q.groups_a;
+    l.spitch = p.spitch;
+    l.kstages = q.kstages;
+    // (at most 65535 x 4 stages of 256: k below 2^26)
+    if ((q.kstages + 3) / 4 > 65535) return FR_ERR_UNSUPPORTED;
+    const dim3 grid(static_cast<unsigned>(q.groups_a + q.groups_b), static_cast<unsigned>((q.kstages + 3) / 4));
+    if (block == 16) fp4_scale_layout_kernel<16><<<grid, 128, 0, st>>>(l);
+    else fp4_scale_layout_kernel<32><<<grid, 128, 0, st>>>(l);
+    FR_CUDA_OK(cudaGetLastError());
+    p.sa = l.da;
+    p.sb = l.db;
+  }
   // split K while the tiles leave at least half of the SMs idle and every CTA keeps a stage
   const DeviceInfo& di = device_info();
-  const int64_t tiles = ta * tb;
+  const int64_t tiles = static_cast<int64_t>(q.tiles_a) * q.tiles_b;
   int split = 1;
   while (split < 8 && tiles * split * 2 <= di.sm_count && split * 2 <= p.kstages) split *= 2;
   p.split = split;
   const int grid = split > 1 ? static_cast<int>(tiles * split) : static_cast<int>(tiles < di.sm_count ? tiles : di.sm_count);
-  CUtensorMap ma, mb;
-  const uint64_t kb = static_cast<uint64_t>(k / 2);
-  int rc = make_tmap_2d(&ma, swapped ? b_q : a_q, p.rows_a, kb, kb, FG_LANES, 128, true, 1);
-  if (rc) return rc;
-  rc = make_tmap_2d(&mb, swapped ? a_q : b_q, p.rows_b, kb, kb, bn, 128, true, 1);
-  if (rc) return rc;
   const bool bf = dtype == FR_BF16;
-  switch (bn) {
+  switch (q.bn) {
     case 32: return launch_fp4_bn<32>(ma, mb, p, block, bf, grid, st);
     case 128: return launch_fp4_bn<128>(ma, mb, p, block, bf, grid, st);
     default: return launch_fp4_bn<256>(ma, mb, p, block, bf, grid, st);

@@ -65,7 +65,8 @@ def quantize_fp4(x: torch.Tensor, block: int = 16, global_scale: torch.Tensor = 
         ws, nbytes = None, 0
         if own:
             nbytes = lib.fr_fp4_quantize_workspace_bytes(mats, rows, cols)
-            ws = _lib.call_workspace(nbytes, dev, "fp4")
+            if nbytes:
+                ws = _lib.call_workspace(nbytes, dev, "fp4")
         rc = lib.fr_fp4_quantize(_lib.ptr(x), _lib.dtype_code(x.dtype), mats, rows, cols,
                                  x.stride(0) if x.dim() == 3 else 0, x.stride(-2) if rows > 1 else cols, block,
                                  _lib.ptr(global_scale), 1 if own else 0, _lib.ptr(q), _lib.ptr(scale), _lib.ptr(ws),
@@ -123,9 +124,12 @@ def matmul_fp4(a_q: torch.Tensor, a_scale: torch.Tensor, b_q: torch.Tensor, b_sc
             out = torch.empty(m, n, dtype=dtype, device=dev)
         if m == 0 or n == 0:
             return out
-        rc = _lib.load().fr_fp4_gemm(_lib.ptr(a_q), _lib.ptr(a_scale), _lib.ptr(a_global), _lib.ptr(b_q), _lib.ptr(b_scale),
-                                     _lib.ptr(b_global), block, m, n, k, _lib.dtype_code(out.dtype), _lib.ptr(out),
-                                     out.stride(0) if m > 1 else n, _lib.stream_ptr(dev))
+        lib = _lib.load()
+        nbytes = lib.fr_fp4_gemm_workspace_bytes(m, n, k, block)
+        ws = _lib.call_workspace(nbytes, dev, "fp4") if nbytes else None
+        rc = lib.fr_fp4_gemm(_lib.ptr(a_q), _lib.ptr(a_scale), _lib.ptr(a_global), _lib.ptr(b_q), _lib.ptr(b_scale),
+                             _lib.ptr(b_global), block, m, n, k, _lib.dtype_code(out.dtype), _lib.ptr(out),
+                             out.stride(0) if m > 1 else n, _lib.ptr(ws), nbytes, _lib.stream_ptr(dev))
     _lib.check(rc, "fr_fp4_gemm")
     return out
 

@@ -299,7 +299,7 @@ int fr_w4a16_dequant(const int32_t* qweight, const void* scales, const int32_t* 
  *   and written, else read; scale = e4m3(amax / (6 * global)), code = e2m1(x * (1 / (scale * global))).  block 32:
  *   scale = 2^(floor(log2 amax) - 2), code = e2m1(x / scale) saturated at 6.  All roundings to nearest even, every
  *   operation a single fp32 rounding.  A block that holds an infinity or a NaN gets a NaN scale and zero codes.
- *   cols must be a multiple of block, mats <= 65535; workspace: fr_fp4_quantize_workspace_bytes, needed with
+ *   cols must be a multiple of block, mats <= 65535; workspace: fr_fp4_quantize_workspace_bytes (0 = none), needed with
  *   own_global only, no initial state.
  * fr_fp4_dequantize: the numbers, rounded to `dtype`; global_scale may be NULL (1). */
 size_t fr_fp4_quantize_workspace_bytes(int64_t mats, int64_t rows, int64_t cols);
@@ -313,10 +313,12 @@ int fr_fp4_dequantize(const void* q, const void* scale, const float* global_scal
  * instructions with fp32 accumulation; c in FR_F16 / FR_BF16 (row pitch ldc), rounded once.  a and b are dense rows as
  * fr_fp4_quantize writes them (mats = 1), both with the same block size; the global scales are one fp32 each on the
  * device, NULL = 1.  k must be a multiple of 32, the codes 16-byte aligned.  A row whose scales hold a NaN gives NaN in
- * its row (column) of c only. */
+ * its row (column) of c only.  workspace (16-byte aligned, no initial state): fr_fp4_gemm_workspace_bytes, 0 for at
+ * most 128 tokens (m), about the size of the scales above that. */
+size_t fr_fp4_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k, int block);
 int fr_fp4_gemm(const void* a_q, const void* a_scale, const float* a_global, const void* b_q, const void* b_scale,
                 const float* b_global, int block, int64_t m, int64_t n, int64_t k, int dtype, void* c, int64_t ldc,
-                void* stream);
+                void* workspace, size_t workspace_bytes, void* stream);
 
 /* The whole layer for at most FR_DECODE_MAX_TOKENS tokens in one cooperative launch: the contract of fr_moe_layer
  * (routing ties to the lower expert id, softmax by the same recipe) with 16-bit or 4-bit expert weights.

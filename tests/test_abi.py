@@ -158,10 +158,14 @@ def test_fp4_oracle_rounds_to_the_nearest_code(block):
 def test_fp4_product_checks_reject_before_any_launch(lib):
     null, p = ctypes.c_void_p(None), ctypes.c_void_p(1 << 20)
 
-    def gemm(m=4, n=8, k=64, block=16, dtype=1, a=p, c=p, ldc=8):
-        return lib.fr_fp4_gemm(a, p, null, p, p, null, block, m, n, k, dtype, c, ldc, null)
+    def gemm(m=4, n=8, k=64, block=16, dtype=1, a=p, c=p, ldc=8, ws=null, nbytes=0):
+        return lib.fr_fp4_gemm(a, p, null, p, p, null, block, m, n, k, dtype, c, ldc, ws, nbytes, null)
     assert gemm(m=-1) == -1 and gemm(k=0) == -1 and gemm(block=8) == -1 and gemm(ldc=7) == -1
     assert gemm(a=null) == -1 and gemm(c=null) == -1
     assert gemm(k=48) == -2 and gemm(dtype=2) == -2 and gemm(m=1 << 32) == -2
     assert gemm(a=ctypes.c_void_p((1 << 20) + 8)) == -3
     assert gemm(m=0) == 0 and gemm(n=0) == 0
+    need = lib.fr_fp4_gemm_workspace_bytes(200, 8, 64, 16)
+    assert need == (2 + 2) * 2048 and lib.fr_fp4_gemm_workspace_bytes(128, 8, 64, 16) == 0
+    assert gemm(m=200) == -4 and gemm(m=200, ws=p, nbytes=need - 1) == -4
+    assert gemm(m=200, ws=ctypes.c_void_p((1 << 20) + 8), nbytes=need) == -3
