@@ -21,6 +21,7 @@
 //
 // The eight warps of a CTA split K; their partial sums meet in shared memory in warp order, so results do not depend
 // on timing.  fp32 accumulation throughout; the activations between the two products are rounded to the 16-bit type.
+#include <algorithm>
 #include <atomic>
 
 #include "fr_common.cuh"
@@ -31,8 +32,13 @@ constexpr int kDecTokens = FR_DECODE_MAX_TOKENS;   // 16: the row side of the MM
 constexpr int kDecMaxExperts = 256;
 constexpr int kDecWarps = 8;
 constexpr int kDecThreads = 32 * kDecWarps;
-constexpr int kDecStages = 2;
-constexpr int kDecStageBytes = 4096;               // per warp: 32 chunks of 128 bytes of a weight row
+constexpr int kDecCodeBytes = 4096;                // of a stage, per warp: 32 chunks of 128 bytes of a weight row
+constexpr int kDecScaleBytes = 512;                // and, for 4-bit weights, 32 chunks' block scales
+
+// Control words of a workspace: zero before the first call, kept up by every call (the CTA that finishes last adds what
+// the call used, so nothing has to be cleared in between).
+enum { DC_COUNT = 0, DC_BASE = 1, DC_FINISHED = 2, DC_BUDGET = 3, DC_EPOCH = 4 };
+constexpr uint32_t kDecPolls = 1u << 22;           // about a second, unless DC_BUDGET holds another limit
 
 enum { WF_16BIT = 0, WF_NV4 = 1, WF_MX4 = 2 };
 
@@ -45,33 +51,74 @@ struct DecodeParams {
   const uint8_t *s1, *s2;        // block scales
   const float *g1, *g2;          // one fp32 scale per expert, or null
   int M, H, I, E, topk, renormalize;
+  int scale_copy1, scale_copy2;  // bytes per cp.async of w1's / w2's scales: 16, 8 or 4; 0: rows start anywhere
   int tokens_per_unit;           // router: tokens one CTA takes for one expert
   uint16_t* out;
   float* tw;
   int32_t* ti;
-  unsigned int* barrier;
-  float* logits;                 // [M, E]
+  unsigned int* control;         // DC_* below
+  unsigned long long* logits;    // [M, E]: fp32 bits below, the call's tag above
   uint16_t* act;                 // [active expert][M][I]
 };
 
-// HI: more than 8 tokens.  Then there is room for one buffer of partial sums only (two CTAs share an SM).
-template <bool HI>
+// 16-bit weights: two CTAs per SM with 128 registers a thread; 4-bit weights: one with 255, the expansion needs them (two
+// CTAs of it, with spills: 109 instead of 94 us for 1 token of 8 experts).  HI: more than 8 tokens.
+template <int WF, bool HI>
+struct DecodeCfg {
+  static constexpr bool TWO = WF == WF_16BIT;
+  static constexpr int STAGES = 2;                  // FIFO depth (four were 3 % slower: requests queue in the memory system)
+  static constexpr int STAGE = TWO ? kDecCodeBytes : kDecCodeBytes + kDecScaleBytes;
+  static constexpr int NS2 = 2, LN2 = 2;            // GEMM2: sub-tiles of 8 rows, and 128-byte lines of a row per stage
+  static constexpr int TOKENS = HI ? 16 : 8;
+  static constexpr int STRIDE = HI ? 20 : 12;       // floats per weight row of a partial tile: conflict-free stores
+  static constexpr int PBUFS = TWO && HI ? 1 : 2;   // buffers of partial sums in turn: one barrier per tile instead of two
+};
+template <int WF, bool HI>
 struct DecodeSmem {
-  static constexpr int kTokens = HI ? 16 : 8;
-  static constexpr int kStride = HI ? 20 : 12;      // floats per weight row of a partial tile: conflict-free stores
-  static constexpr int kBufs = HI ? 1 : 2;          // two buffers in turn: one barrier per tile instead of two
-  uint8_t ring[kDecWarps][kDecStages][kDecStageBytes];
-  float part[kBufs][kDecWarps][32 * kStride];
-  float weight[kDecMaxExperts][kTokens];      // routing weight by slot (position in `list`) and token
+  using C = DecodeCfg<WF, HI>;
+  uint8_t ring[kDecWarps][C::STAGES][C::STAGE];
+  float part[C::PBUFS][kDecWarps][32 * C::STRIDE];
+  float weight[kDecMaxExperts][C::TOKENS];    // routing weight by slot (position in `list`) and token
   uint32_t mask[kDecMaxExperts];              // by expert: bit t = token t goes there; upper half: its slot
   uint16_t list[kDecMaxExperts];              // active experts in ascending order
   uint32_t scan[kDecWarps];
+  uint32_t base, epoch;                       // of the control words, read once
+  int ok;
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t size) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// the scales of 128 bytes of codes of one row (16 bytes, or 8 for blocks of 32), `left` bytes of the row remaining;
+// what lies past the row's end becomes zero
+template <int BYTES>
+__device__ __forceinline__ void cp_async_scales(uint32_t dst, const uint8_t* src, int left, int unit) {
+  if (unit == 0) {                 // rows that start anywhere: byte by byte, at once
+#pragma unroll
+    for (int i = 0; i < BYTES; i += 4) {
+      uint32_t v = 0;
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        if (i + b < left) v |= static_cast<uint32_t>(__ldg(src + i + b)) << (8 * b);
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + i), "r"(v) : "memory");
+    }
+  } else if (BYTES == 16 && unit == 16) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(min(max(left, 0), 16)) : "memory");
+  } else if (unit >= 8) {
+#pragma unroll
+    for (int i = 0; i < BYTES; i += 8)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst + i), "l"(left > i ? src + i : src),
+                   "r"(min(max(left - i, 0), 8))
+                   : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < BYTES; i += 4)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + i), "l"(left > i ? src + i : src),
+                   "r"(min(max(left - i, 0), 4))
+                   : "memory");
+  }
+}
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
@@ -80,12 +127,12 @@ __device__ __forceinline__ void cp_async_wait() {
 template <bool BF16>
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (BF16)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -119,6 +166,16 @@ struct Fp4Expand {
       }
     }
   }
+  static __device__ __forceinline__ void order(const uint4& u, uint32_t (&r)[4]) {
+    if constexpr (BF16) {            // pairs (j, j + 4)
+      r[0] = __byte_perm(u.x, u.z, 0x5410);
+      r[1] = __byte_perm(u.x, u.z, 0x7632);
+      r[2] = __byte_perm(u.y, u.w, 0x5410);
+      r[3] = __byte_perm(u.y, u.w, 0x7632);
+    } else {
+      r[0] = u.x, r[1] = u.y, r[2] = u.z, r[3] = u.w;
+    }
+  }
   static __device__ __forceinline__ uint32_t mul(uint32_t a, uint32_t m) {
     uint32_t r;
     if constexpr (BF16) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(m));
@@ -142,64 +199,84 @@ struct Fp4Expand {
   }
 };
 
-// One token row's operand for the 64 bytes of weights a quad holds: `p` points at the lane's first element.
-// 16-bit weights: 8 elements; 4-bit: 32 elements, for bf16 reordered to the pairs (j, j + 4) that Fp4Expand makes.  ANY
-// false: the row is known to be absent (tokens 8-15 of a batch of at most 8).
-template <bool BF16, int WF, bool ANY = true>
-__device__ __forceinline__ void load_tokens(const uint16_t* p, bool valid, bool coherent, uint32_t (&r)[WF == WF_16BIT ? 4 : 16]) {
-  constexpr int NV = WF == WF_16BIT ? 1 : 4;
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (ANY && valid) u = coherent ? __ldcg(reinterpret_cast<const uint4*>(p) + v) : __ldg(reinterpret_cast<const uint4*>(p) + v);
-    if constexpr (WF == WF_16BIT || !BF16) {
-      r[4 * v] = u.x, r[4 * v + 1] = u.y, r[4 * v + 2] = u.z, r[4 * v + 3] = u.w;
-    } else {
-      r[4 * v] = __byte_perm(u.x, u.z, 0x5410);
-      r[4 * v + 1] = __byte_perm(u.x, u.z, 0x7632);
-      r[4 * v + 2] = __byte_perm(u.y, u.w, 0x5410);
-      r[4 * v + 3] = __byte_perm(u.y, u.w, 0x7632);
-    }
-  }
-}
-
-// acc += tokens * weights for one 16-byte chunk per lane
-template <bool BF16, int WF>
-__device__ __forceinline__ void chunk_mma(float (&acc)[4], const uint4& w, uint32_t scales,
-                                          const uint32_t (&lo)[WF == WF_16BIT ? 4 : 16],
-                                          const uint32_t (&hi)[WF == WF_16BIT ? 4 : 16]) {
-  if constexpr (WF == WF_16BIT) {
-    const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]}, a1[4] = {lo[2], hi[2], lo[3], hi[3]};
-    mma_16816<BF16>(acc, a0, w.x, w.y);
-    mma_16816<BF16>(acc, a1, w.z, w.w);
-  } else {
-    using X = Fp4Expand<BF16, WF>;
-    uint32_t m[2];
-    X::mult(scales, m);
-    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t o[4];
-      X::expand(ww[i], m[i >> 1], o);
-      const uint32_t a0[4] = {lo[4 * i], hi[4 * i], lo[4 * i + 1], hi[4 * i + 1]};
-      const uint32_t a1[4] = {lo[4 * i + 2], hi[4 * i + 2], lo[4 * i + 3], hi[4 * i + 3]};
-      mma_16816<BF16>(acc, a0, o[0], o[1]);
-      mma_16816<BF16>(acc, a1, o[2], o[3]);
-    }
-  }
-}
-
-// the scale bytes of a lane's 16 bytes of codes
+// One token row's operand for the 64 bytes of weights a quad holds (16-bit weights: the lane's 8 elements, 4-bit: 32);
+// `p` points at the lane's first element.  Where `valid` is false the registers keep what they held: zeros, or earlier
+// elements of the same token.  Past the end of a row they meet weights of zero (and a NaN among them has made the
+// token's sum NaN already); for a token the expert does not get, the sums are not used.
 template <int WF>
-__device__ __forceinline__ uint32_t load_scales(const uint8_t* at, bool valid) {
-  if (!valid) return 0;
-  if constexpr (WF == WF_NV4) return __ldg(reinterpret_cast<const uint16_t*>(at));
-  return __ldg(at);
+__device__ __forceinline__ void load_tokens(const uint16_t* p, bool valid, uint4 (&r)[WF == WF_16BIT ? 1 : 4]) {
+  if (!valid) return;
+#pragma unroll
+  for (int v = 0; v < (WF == WF_16BIT ? 1 : 4); ++v) r[v] = *(reinterpret_cast<const uint4*>(p) + v);
 }
+
+// acc += tokens * weights for one 16-byte chunk per lane of 16-bit weights
+template <bool BF16>
+__device__ __forceinline__ void chunk_mma(float (&acc)[4], const uint4& w, const uint4& lo, const uint4& hi) {
+  const uint32_t a0[4] = {lo.x, hi.x, lo.y, hi.y}, a1[4] = {lo.z, hi.z, lo.w, hi.w};
+  mma_16816<BF16>(acc, a0, w.x, w.y);
+  mma_16816<BF16>(acc, a1, w.z, w.w);
+}
+
+// the same for NS sub-tiles of 4-bit weights: word by word, so that the sub-tiles' products are independent
+template <bool BF16, int WF, int NS>
+__device__ __forceinline__ void chunk_mma4(float (&acc)[NS][4], const uint4 (&w)[NS], const uint32_t (&scales)[NS],
+                                           const uint4 (&lo)[4], const uint4 (&hi)[4]) {
+  using X = Fp4Expand<BF16, WF>;
+  uint32_t m[NS][2];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) X::mult(scales[s], m[s]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    // a word's eight elements as four registers, in the order Fp4Expand gives the codes
+    uint32_t l[4], h[4];
+    X::order(lo[i], l);
+    X::order(hi[i], h);
+    const uint32_t a0[4] = {l[0], h[0], l[1], h[1]}, a1[4] = {l[2], h[2], l[3], h[3]};
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const uint32_t word = i == 0 ? w[s].x : i == 1 ? w[s].y : i == 2 ? w[s].z : w[s].w;
+      uint32_t o[4];
+      X::expand(word, m[s][i >> 1], o);
+      mma_16816<BF16>(acc[s], a0, o[0], o[1]);
+      mma_16816<BF16>(acc[s], a1, o[2], o[3]);
+    }
+  }
+}
+
+// One stage (LN lines of 128 bytes of every row of NS sub-tiles) of 4-bit weights, in half lines with two operand buffers
+// in turn: `fetch(st)` requests the operand of the half line after st into the buffer that st does not use, `stage` waits
+// for the weights and says where the lane's first chunk and scales are.
+template <bool BF16, int WF, int NS, int LN, class Fetch, class Stage>
+__device__ __forceinline__ void full_step4(float (&acc)[NS][4], const uint4 (&lo)[2][4], const uint4 (&hi)[2][4],
+                                           Fetch fetch, Stage stage) {
+  constexpr int SCB = WF == WF_NV4 ? 16 : 8;
+  const uint8_t* at = nullptr;
+  const uint8_t* sc_at = nullptr;
+#pragma unroll
+  for (int st = 0; st < 2 * LN; ++st) {
+    fetch(st);
+    if (st == 0) stage(at, sc_at);
+    const uint8_t* half = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(at) ^ ((st & 1) << 6)) + (st >> 1) * NS * 1024;
+    uint4 w[NS];
+    uint32_t sc[NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      w[s] = *reinterpret_cast<const uint4*>(half + s * 1024);
+      const uint8_t* q = sc_at + (s + (st >> 1) * NS) * 8 * SCB + (st & 1) * (SCB / 2);
+      sc[s] = WF == WF_NV4 ? *reinterpret_cast<const uint16_t*>(q) : *q;
+    }
+    chunk_mma4<BF16, WF, NS>(acc, w, sc, lo[st & 1], hi[st & 1]);
+  }
+}
+
+struct DecodeStep {     // GEMM2: a double step of one active expert
+  int slot, b;
+};
 
 // ---- router: logits of all (token, expert) pairs, spread over the grid --------------------------------------
 template <bool BF16>
-__device__ __forceinline__ void decode_logits(const DecodeParams& p, float* red /* [kDecWarps][kDecTokens] */) {
+__device__ __forceinline__ void decode_logits(const DecodeParams& p, uint32_t tag, float* red /* [kDecWarps][kDecTokens] */) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tpu = p.tokens_per_unit, groups = (p.M + tpu - 1) / tpu;
   for (int u = blockIdx.x; u < p.E * groups; u += gridDim.x) {
@@ -248,7 +325,9 @@ __device__ __forceinline__ void decode_logits(const DecodeParams& p, float* red 
 #pragma unroll
       for (int w = 0; w < kDecWarps; ++w) v += red[w * kDecTokens + threadIdx.x];
       if (v != v) v = -INFINITY;       // NaN ranks last, as in the other routers
-      p.logits[static_cast<int64_t>(t0 + threadIdx.x) * p.E + e] = v;
+      // value and tag in one 8-byte store: a reader that sees the tag has the value, no fence or barrier in between
+      p.logits[static_cast<int64_t>(t0 + threadIdx.x) * p.E + e] =
+          (static_cast<unsigned long long>(tag) << 32) | __float_as_uint(v);
     }
     __syncthreads();
   }
@@ -259,68 +338,102 @@ __device__ __forceinline__ uint32_t order_key(float v) {   // larger value, larg
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Every CTA ranks all tokens: one warp per token, k rounds of arg-max (equal logits: lower expert id), softmax by the
-// fixed fp32 recipe of the routers.  `sel` / `val`: [kDecTokens][E] scratch.
-template <bool HI>
-__device__ __forceinline__ void decode_rank(const DecodeParams& p, DecodeSmem<HI>& sm, uint16_t* sel, float* val) {
+// Every CTA ranks all tokens: a warp polls the logits of its (up to two) tokens until all carry this call's tag
+// (bounded), then k rounds of arg-max (equal logits: lower expert id), softmax by the fixed fp32 recipe of the routers.
+// `sel` / `val`: [kDecTokens][E] scratch.  False: the logits did not arrive in time.
+template <class Smem, int NT>
+__device__ __forceinline__ bool decode_rank(const DecodeParams& p, Smem& sm, uint32_t tag, uint16_t* sel, float* val) {
+  constexpr int NE = kDecMaxExperts / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int e = threadIdx.x; e < p.E; e += kDecThreads) sm.mask[e] = 0;
   __syncthreads();
-  for (int t = warp; t < p.M; t += kDecWarps) {
-    const float* l = p.logits + static_cast<int64_t>(t) * p.E;
-    uint16_t* my_sel = sel + t * p.E;
-    float* my_val = val + t * p.E;
-    float v[kDecMaxExperts / 32];
-    uint32_t key[kDecMaxExperts / 32];
+  if (warp < p.M) {
+    float v[NT][NE];
+    uint32_t key[NT][NE];
+    bool all = false;
+    const uint32_t asked = __ldcg(p.control + DC_BUDGET), budget = asked ? asked : kDecPolls;
+    for (uint32_t poll = 0; poll <= budget && !all; ++poll) {
+      unsigned long long u[NT][NE];
 #pragma unroll
-    for (int i = 0; i < kDecMaxExperts / 32; ++i) {
-      const int c = i * 32 + lane;
-      v[i] = c < p.E ? __ldcg(l + c) : 0.0f;
-      key[i] = c < p.E ? order_key(v[i]) : 0u;
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+          const int t = warp + n * kDecWarps, c = i * 32 + lane;
+          u[n][i] = static_cast<unsigned long long>(tag) << 32;
+          if (i * 32 < p.E && t < p.M && c < p.E)
+            asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(u[n][i]) : "l"(p.logits + static_cast<int64_t>(t) * p.E + c));
+        }
+      bool mine = true;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+          mine &= static_cast<uint32_t>(u[n][i] >> 32) == tag;
+          v[n][i] = __uint_as_float(static_cast<uint32_t>(u[n][i]));
+          key[n][i] = i * 32 + lane < p.E ? order_key(v[n][i]) : 0u;
+        }
+      all = __all_sync(0xffffffffu, mine);
     }
-    for (int j = 0; j < p.topk; ++j) {
-      uint32_t best = 0;
-      int at = 0;
-      float bv = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kDecMaxExperts / 32; ++i)
-        if (key[i] > best) best = key[i], at = i, bv = v[i];
-      const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-      const uint32_t col = __reduce_min_sync(0xffffffffu, best == top ? static_cast<uint32_t>(at * 32 + lane) : 0xFFFFu);
-      if (col == static_cast<uint32_t>(at * 32 + lane)) {
-        my_sel[j] = static_cast<uint16_t>(col);
-        my_val[j] = bv;
-        atomicOr(&sm.mask[col], 1u << t);
-#pragma unroll
-        for (int i = 0; i < kDecMaxExperts / 32; ++i)
-          if (i == at) key[i] = 0;
-      }
-      __syncwarp();
+    if (!all && lane == 0) {
+      report(ST_WAIT_TIMEOUT, 0x800);
+      sm.ok = 0;
     }
-    const float top = my_val[0];
-    float s = 0.0f;
-    if (p.renormalize) {
-      for (int j = 0; j < p.topk; ++j) {
-        const float ej = exp_recipe(__fsub_rn(my_val[j], top));
-        s = (j == 0) ? ej : __fadd_rn(s, ej);
-      }
-    } else {
+    for (int j = 0; j < p.topk && all; ++j) {
 #pragma unroll
-      for (int i = 0; i < kDecMaxExperts / 32; ++i)
-        if (i * 32 + lane < p.E) s += exp_recipe(__fsub_rn(v[i], top));
-      for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+      for (int n = 0; n < NT; ++n) {
+        const int t = warp + n * kDecWarps;
+        uint32_t best = 0;
+        int at = 0;
+        float bv = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NE; ++i)
+          if (i * 32 < p.E && key[n][i] > best) best = key[n][i], at = i, bv = v[n][i];
+        const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+        const uint32_t col = __reduce_min_sync(0xffffffffu, best == top ? static_cast<uint32_t>(at * 32 + lane) : 0xFFFFu);
+        if (t < p.M && col == static_cast<uint32_t>(at * 32 + lane)) {
+          sel[t * p.E + j] = static_cast<uint16_t>(col);
+          val[t * p.E + j] = bv;
+          atomicOr(&sm.mask[col], 1u << t);
+#pragma unroll
+          for (int i = 0; i < NE; ++i)
+            if (i == at) key[n][i] = 0;
+        }
+      }
     }
     __syncwarp();
-    for (int j = lane; j < p.topk; j += 32) {
-      const float w = __fdiv_rn(exp_recipe(__fsub_rn(my_val[j], top)), s);
-      my_val[j] = w;
-      if (blockIdx.x == 0 && p.tw) {
-        p.tw[static_cast<int64_t>(t) * p.topk + j] = w;
-        p.ti[static_cast<int64_t>(t) * p.topk + j] = my_sel[j];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int t = warp + n * kDecWarps;
+      if (t >= p.M || !all) break;
+      float* my_val = val + t * p.E;
+      const float top = my_val[0];
+      float s = 0.0f;
+      if (!p.renormalize) {
+#pragma unroll
+        for (int i = 0; i < NE; ++i)
+          if (i * 32 + lane < p.E) s += exp_recipe(__fsub_rn(v[n][i], top));
+        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+      }
+      __syncwarp();
+      for (int j = lane; j < p.topk; j += 32) my_val[j] = exp_recipe(__fsub_rn(my_val[j], top));
+      __syncwarp();
+      if (p.renormalize) {                 // in the order of the ranks
+        s = my_val[0];
+        for (int j = 1; j < p.topk; ++j) s = __fadd_rn(s, my_val[j]);
+      }
+      __syncwarp();
+      for (int j = lane; j < p.topk; j += 32) {
+        const float w = __fdiv_rn(my_val[j], s);
+        my_val[j] = w;
+        if (blockIdx.x == 0 && p.tw) {
+          p.tw[static_cast<int64_t>(t) * p.topk + j] = w;
+          p.ti[static_cast<int64_t>(t) * p.topk + j] = sel[t * p.E + j];
+        }
       }
     }
   }
   __syncthreads();
+  if (!sm.ok) return false;
   // active experts in ascending order; `scan` holds the warps' counts
   const bool active = threadIdx.x < p.E && sm.mask[threadIdx.x] != 0;
   const uint32_t vote = __ballot_sync(0xffffffffu, active);
@@ -340,21 +453,45 @@ __device__ __forceinline__ void decode_rank(const DecodeParams& p, DecodeSmem<HI
     sm.weight[sm.mask[sel[t * p.E + j]] >> 16][t] = val[t * p.E + j];
   }
   __syncthreads();
+  return true;
+}
+
+// The CTA's last act: whoever is last of the grid moves the control words on for the next call.
+__device__ __forceinline__ void decode_finish(const DecodeParams& p, uint32_t base, uint32_t epoch) {
+  if (threadIdx.x != 0) return;
+  __threadfence();
+  if (atomicAdd(p.control + DC_FINISHED, 1u) == gridDim.x - 1) {
+    p.control[DC_FINISHED] = 0;
+    p.control[DC_BASE] = base + gridDim.x;
+    p.control[DC_EPOCH] = epoch + 1;
+  }
 }
 
 template <bool BF16, int WF, bool HI>
-__global__ void __launch_bounds__(kDecThreads, 2) moe_decode_kernel(const DecodeParams p) {
+__global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1)) moe_decode_kernel(const DecodeParams p) {
   extern __shared__ __align__(128) uint8_t dec_smem[];
-  using Smem = DecodeSmem<HI>;
+  using C = DecodeCfg<WF, HI>;
+  using Smem = DecodeSmem<WF, HI>;
   Smem& sm = *reinterpret_cast<Smem*>(dec_smem);
-  constexpr int PS = Smem::kStride;
+  constexpr int PS = C::STRIDE;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
   const unsigned int G = gridDim.x;
 
-  decode_logits<BF16>(p, &sm.part[0][0][0]);
-  if (!grid_barrier(p.barrier, G)) return;
-  decode_rank(p, sm, reinterpret_cast<uint16_t*>(&sm.part[0][0][0]), reinterpret_cast<float*>(&sm.ring[0][0][0]));
+  if (threadIdx.x == 0) {
+    sm.base = __ldcg(p.control + DC_BASE);
+    sm.epoch = __ldcg(p.control + DC_EPOCH);
+    sm.ok = 1;
+  }
+  __syncthreads();
+  const uint32_t base = sm.base, epoch = sm.epoch;
+  decode_logits<BF16>(p, epoch + 1, &sm.part[0][0][0]);
+  if (!decode_rank<Smem, HI ? 2 : 1>(p, sm, epoch + 1, reinterpret_cast<uint16_t*>(&sm.part[0][0][0]),
+                   reinterpret_cast<float*>(&sm.ring[0][0][0]))) {
+    if (threadIdx.x == 0) atomicAdd(p.control + DC_COUNT, 1u);      // the others' barrier counts every CTA
+    decode_finish(p, base, epoch);
+    return;
+  }
   int n_active = 0;
   for (int w = 0; w < kDecWarps; ++w) n_active += sm.scan[w];
 
@@ -373,7 +510,8 @@ __global__ void __launch_bounds__(kDecThreads, 2) moe_decode_kernel(const Decode
   // A step is 128 bytes (a full line) of every row of a tile.  GEMM1: tiles of 16 pairs = four sub-tiles of 4 SiLU + 4
   // linear rows, warp w takes steps w, w + 8, ...; GEMM2: tiles of 16 rows = two sub-tiles of 8, two steps at a time,
   // the double steps of all active experts in one sequence dealt to the warps in turn.
-  const int nb1 = (rb1 + 127) / 128, nb2 = (rb2 + 255) / 256;
+  constexpr int NS2 = C::NS2, LN2 = C::LN2;
+  const int nb1 = (rb1 + 127) / 128, nb2 = (rb2 + 128 * LN2 - 1) / (128 * LN2);
 
   // ---- the loading end of the stream: one segment = one row tile of GEMM1, or one (row tile, expert) of GEMM2 ----
   // Warp w's steps of a segment are b0, b0 + 8, ...; ld_rem counts those still to be requested.  Eight lanes copy one
@@ -389,7 +527,14 @@ __global__ void __launch_bounds__(kDecThreads, 2) moe_decode_kernel(const Decode
   // chunk c of row r sits at position c ^ 4 * (r & 1) of the row: the reads below then touch every bank once
   const uint32_t ring = smem_u32(&sm.ring[warp][0][0]) + cr * 128 + ((cc ^ ((cr & 1) << 2)) << 4);
   uint32_t ld_at = 0, at_off = 0;
-  constexpr uint32_t RING = kDecStages * kDecStageBytes;
+  constexpr uint32_t STAGE = C::STAGE;
+  constexpr int kDecStages = C::STAGES;
+  // 4-bit weights: lane r copies the scales of chunk r of the stage (row r, or row r & 15 of line r >> 4)
+  constexpr int SCB = WF == WF_NV4 ? 16 : 8;
+  const uint8_t* ld_sc = nullptr;
+  int ld_sc_left = 0;
+  bool ld_sc_ok = false;
+  const uint32_t sc_ring = smem_u32(&sm.ring[warp][0][0]) + kDecCodeBytes + lane * SCB;
   const int64_t lin1 = static_cast<int64_t>(p.I) * rb1;     // from a SiLU row to its linear row
   auto issue = [&]() {
     while (ld_rem == 0) {              // next segment; the loop is for segments that have no step for this warp
@@ -400,21 +545,33 @@ __global__ void __launch_bounds__(kDecThreads, 2) moe_decode_kernel(const Decode
         ld_src = p.w1 + row * rb1 + ld_k;
         ld_rows = cnt - cr;
         ld_rem = warp < nb1 ? (nb1 - warp + kDecWarps - 1) / kDecWarps : 0;
+        if constexpr (WF != WF_16BIT) {
+          const int pair = 4 * (lane >> 3) + (lane & 3);
+          ld_sc_ok = pair < cnt;
+          ld_sc_left = sb1 - warp * SCB;
+          ld_sc = p.s1 + (static_cast<int64_t>(sm.list[ld_a]) * 2 * p.I + ld_j + pair + ((lane & 4) ? p.I : 0)) * sb1 + warp * SCB;
+        }
         ld_left -= cnt;
         ld_j += cnt;
         if (ld_j == p.I) ld_j = 0, ++ld_a;
       } else if (ld_row < row1) {
         ld_second = true;
         const int64_t row = static_cast<int64_t>(sm.list[ld_slot]) * p.H + ld_row + cr;
-        ld_k = ld_b2 * 256 + cc * 16;
+        ld_k = ld_b2 * (128 * LN2) + cc * 16;
         ld_src = p.w2 + row * rb2 + ld_k;
         ld_rows = row1 - ld_row - cr;
         if (ld_b2 < nb2) ld_rem = (nb2 - ld_b2 + kDecWarps - 1) / kDecWarps;
+        if constexpr (WF != WF_16BIT) {
+          const int off = (ld_b2 * 2 + (lane >> 4)) * SCB;
+          ld_sc_ok = ld_row + (lane & 15) < row1;
+          ld_sc_left = sb2 - off;
+          ld_sc = p.s2 + (static_cast<int64_t>(sm.list[ld_slot]) * p.H + ld_row + (lane & 15)) * sb2 + off;
+        }
         ld_b2 += ld_rem * kDecWarps - nb2;
         if (++ld_slot == n_active) {
           ld_slot = 0;
           ld_b2 = warp;
-          ld_row += 16;
+          ld_row += 8 * NS2;
         }
       } else {
         cp_async_commit();
@@ -436,33 +593,43 @@ __global__ void __launch_bounds__(kDecThreads, 2) moe_decode_kernel(const Decode
       }
       ld_k += kDecWarps * 128;
       ld_src += kDecWarps * 128;
+      if constexpr (WF != WF_16BIT) {
+        if (ld_sc_ok) cp_async_scales<SCB>(sc_ring + ld_at, ld_sc_left > 0 ? ld_sc : p.s1, ld_sc_left, p.scale_copy1);
+        ld_sc += kDecWarps * SCB;
+        ld_sc_left -= kDecWarps * SCB;
+      }
     } else {
-      const uint32_t size0 = ld_k < rb2 ? 16u : 0u, size1 = ld_k + 128 < rb2 ? 16u : 0u;
       const uint8_t* src = ld_src;
       const int64_t step = static_cast<int64_t>(4) * rb2;
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {        // half a sub-tile: 4 rows
+      for (int s = 0; s < 2 * NS2; ++s) {  // half a sub-tile: 4 rows
         if (4 * s < ld_rows) {
-          cp_async16(dst + s * 512, src, size0);
-          cp_async16(dst + s * 512 + 2048, src + 128, size1);
+#pragma unroll
+          for (int l = 0; l < LN2; ++l)
+            cp_async16(dst + s * 512 + l * 2048, src + l * 128, ld_k + l * 128 < rb2 ? 16u : 0u);
         }
         src += step;
       }
-      ld_k += kDecWarps * 256;
-      ld_src += kDecWarps * 256;
+      ld_k += kDecWarps * 128 * LN2;
+      ld_src += kDecWarps * 128 * LN2;
+      if constexpr (WF != WF_16BIT) {
+        if (ld_sc_ok) cp_async_scales<SCB>(sc_ring + ld_at, ld_sc_left > 0 ? ld_sc : p.s2, ld_sc_left, p.scale_copy2);
+        ld_sc += kDecWarps * 2 * SCB;
+        ld_sc_left -= kDecWarps * 2 * SCB;
+      }
     }
     --ld_rem;
     cp_async_commit();
-    ld_at = (ld_at + kDecStageBytes) & (RING - 1);
+    ld_at = ld_at == (kDecStages - 1) * STAGE ? 0 : ld_at + STAGE;
   };
   // the reading end: lane (g, t4) takes chunk t4 + 4 * st of row g of a sub-tile
   const uint8_t* fifo = &sm.ring[warp][0][0] + g * 128 + ((t4 ^ ((g & 1) << 2)) << 4);
-  auto next_stage = [&]() {
+  auto next_stage = [&](const uint8_t*& at, const uint8_t*& sc_at) {
     cp_async_wait<kDecStages - 1>();
     __syncwarp();
-    const uint8_t* at = fifo + at_off;
-    at_off = (at_off + kDecStageBytes) & (RING - 1);
-    return at;
+    at = fifo + at_off;
+    sc_at = &sm.ring[warp][0][0] + at_off + kDecCodeBytes + g * SCB + t4 * (SCB / 8);
+    at_off = at_off == (kDecStages - 1) * STAGE ? 0 : at_off + STAGE;
   };
   auto chunk = [&](const uint8_t* at, int st) {   // st: 0 or 1; the other half of a row is at ^ 64
     return *reinterpret_cast<const uint4*>(st ? reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(at) ^ 64) : at);
@@ -470,13 +637,24 @@ __global__ void __launch_bounds__(kDecThreads, 2) moe_decode_kernel(const Decode
 #pragma unroll
   for (int s = 0; s < kDecStages; ++s) issue();
 
-  constexpr int TR = WF == WF_16BIT ? 4 : 16;
-  constexpr int SPB = WF == WF_NV4 ? 8 : 4;        // scale bytes per 64 bytes of codes
-  int buf = 0;                                     // partial-sum buffer of the current tile
+  constexpr int NV = WF == WF_16BIT ? 1 : 4;
   // ---- GEMM1 + SiLU ----
   {
+    uint4 lo[2][NV] = {}, hi[2][NV] = {};     // of the two halves of a step
+    int buf = 0;
     int64_t left = pair1 - pair0;
     int a = static_cast<int>(pair0 / p.I), j0 = static_cast<int>(pair0 - static_cast<int64_t>(a) * p.I);
+    const uint16_t* const x0 = p.x + static_cast<int64_t>(g) * p.H + (warp * 8 + t4) * ELT;
+    const int64_t x_hi = static_cast<int64_t>(8) * p.H;
+    constexpr int XS = kDecWarps * 8 * ELT;             // elements from a warp's step to its next
+    const int kb0 = warp * 128 + t4 * 16;
+    if constexpr (WF != WF_16BIT) {
+      if (left > 0 && warp < nb1) {
+        const uint32_t mask = sm.mask[sm.list[a]];
+        load_tokens<WF>(x0, ((mask >> g) & 1u) && kb0 < rb1, lo[0]);
+        if constexpr (HI) load_tokens<WF>(x0 + x_hi, ((mask >> (g + 8)) & 1u) && kb0 < rb1, hi[0]);
+      }
+    }
     while (left > 0) {
       const int cnt = static_cast<int>(min(static_cast<int64_t>(min(16, p.I - j0)), left));
       const int e = sm.list[a];
@@ -487,43 +665,49 @@ __global__ void __launch_bounds__(kDecThreads, 2) moe_decode_kernel(const Decode
       for (int s = 0; s < 4; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[s][i] = 0.0f;
-      int kb = warp * 128 + t4 * 16;
-      const uint16_t* xp = p.x + static_cast<int64_t>(g) * p.H + (warp * 8 + t4) * ELT;
-      const int64_t x_hi = static_cast<int64_t>(8) * p.H;
-      const uint8_t* sp = p.s1 + (static_cast<int64_t>(e) * 2 * p.I + (g < 4 ? 0 : p.I) + j0 + (g & 3)) * sb1 +
-                          (WF == WF_NV4 ? kb >> 3 : kb >> 4);
-      const int64_t sb4 = static_cast<int64_t>(4) * sb1;
+      int kb = kb0;
+      const uint16_t* xp = x0;
       for (int b = warp; b < nb1; b += kDecWarps) {
-        uint32_t lo[2][TR], hi[2][TR];
-        const uint8_t* at = nullptr;
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          const bool in = kb + st * 64 < rb1;
-          load_tokens<BF16, WF>(xp + st * 4 * ELT, use_lo && in, false, lo[st]);
-          load_tokens<BF16, WF, HI>(xp + st * 4 * ELT + x_hi, use_hi && in, false, hi[st]);
-          uint32_t sc[4] = {0, 0, 0, 0};
-          if constexpr (WF != WF_16BIT) {
-#pragma unroll
-            for (int s = 0; s < 4; ++s) sc[s] = load_scales<WF>(sp + s * sb4 + st * SPB, 4 * s + (g & 3) < cnt && in);
-          }
-          if (WF == WF_16BIT ? st == 1 : st == 0) at = next_stage();
-          if constexpr (WF != WF_16BIT) {
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-              chunk_mma<BF16, WF>(acc[s], chunk(at + s * 1024, st), sc[s], lo[st], hi[st]);
-          }
-        }
         if constexpr (WF == WF_16BIT) {
 #pragma unroll
-          for (int s = 0; s < 4; ++s)
+          for (int st = 0; st < 2; ++st) {
+            const bool in = kb + st * 64 < rb1;
+            load_tokens<WF>(xp + st * 4 * ELT, use_lo && in, lo[st]);
+            if constexpr (HI) load_tokens<WF>(xp + st * 4 * ELT + x_hi, use_hi && in, hi[st]);
+          }
+          const uint8_t *at, *no_scales;
+          next_stage(at, no_scales);
 #pragma unroll
-            for (int st = 0; st < 2; ++st) chunk_mma<BF16, WF>(acc[s], chunk(at + s * 1024, st), 0, lo[st], hi[st]);
+          for (int st = 0; st < 2; ++st)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) chunk_mma<BF16>(acc[s], chunk(at + s * 1024, st), lo[st][0], hi[st][0]);
+        } else {
+          auto fetch = [&](int st) {
+            const uint16_t* np = xp + 4 * ELT;
+            bool in = kb + 64 < rb1, nl = use_lo, nh = use_hi;
+            if (st == 1) {
+              if (b + kDecWarps < nb1) {
+                np = xp + XS;
+                in = kb + kDecWarps * 128 < rb1;
+              } else {                       // the next tile's first step
+                np = x0;
+                in = kb0 < rb1 && left > cnt;
+                if (in && j0 + cnt == p.I) {
+                  const uint32_t m2 = sm.mask[sm.list[a + 1]];
+                  nl = (m2 >> g) & 1u;
+                  nh = (m2 >> (g + 8)) & 1u;
+                }
+              }
+            }
+            load_tokens<WF>(np, nl && in, lo[st ^ 1]);
+            if constexpr (HI) load_tokens<WF>(np + x_hi, nh && in, hi[st ^ 1]);
+          };
+          full_step4<BF16, WF, 4, 1>(acc, lo, hi, fetch, next_stage);
         }
         __syncwarp();
         issue();
         kb += kDecWarps * 128;
-        xp += kDecWarps * 8 * ELT;
-        sp += kDecWarps * 2 * SPB;
+        xp += XS;
       }
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
@@ -555,22 +739,42 @@ __global__ void __launch_bounds__(kDecThreads, 2) moe_decode_kernel(const Decode
           p.act[(static_cast<int64_t>(a) * p.M + t) * p.I + j0 + j] = static_cast<uint16_t>(v);
         }
       }
-      if constexpr (Smem::kBufs == 2) buf ^= 1;
+      if constexpr (C::PBUFS == 2) buf ^= 1;
       else __syncthreads();
       left -= cnt;
       j0 += cnt;
       if (j0 == p.I) j0 = 0, ++a;
     }
   }
-  if (!grid_barrier(p.barrier, G)) {
+  // ---- every activation is written and visible ----
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p.control + DC_COUNT) : "memory");
+    const uint32_t asked = __ldcg(p.control + DC_BUDGET), budget = asked ? asked : kDecPolls;
+    uint32_t poll = 0, seen;
+    while (true) {
+      asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(p.control + DC_COUNT) : "memory");
+      if (seen - base >= G) break;
+      if (++poll > budget) {
+        report(ST_WAIT_TIMEOUT, 0x802);
+        sm.ok = 0;
+        break;
+      }
+    }
+  }
+  __syncthreads();
+  if (!sm.ok) {
     cp_async_wait<0>();
+    decode_finish(p, base, epoch);
     return;
   }
   // ---- GEMM2 + weighted sum over the experts ----
-  for (int r0 = row0; r0 < row1; r0 += 16) {
-    float tot[2][4], acc[2][4];
+  for (int r0 = row0; r0 < row1; r0 += 8 * NS2) {
+    constexpr int NT = WF == WF_16BIT ? 4 : 2;
+    uint4 lo[NT][NV] = {}, hi[NT][NV] = {};
+    float tot[NS2][4], acc[NS2][4];
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int s = 0; s < NS2; ++s)
 #pragma unroll
       for (int i = 0; i < 4; ++i) tot[s][i] = acc[s][i] = 0.0f;
     // An expert's sum enters a token's total only where the token is routed to it: an infinity or NaN in its weights
@@ -580,9 +784,9 @@ __global__ void __launch_bounds__(kDecThreads, 2) moe_decode_kernel(const Decode
       const uint32_t mask = sm.mask[e];
       float f = 1.0f;
       if constexpr (WF != WF_16BIT) f = (p.g2 ? __ldg(p.g2 + e) : 1.0f) * Fp4Expand<BF16, WF>::kUnit;
-      const float w_lo = sm.weight[from][g] * f, w_hi = HI ? sm.weight[from][(g + 8) % Smem::kTokens] * f : 0.0f;
+      const float w_lo = sm.weight[from][g] * f, w_hi = HI ? sm.weight[from][(g + 8) % C::TOKENS] * f : 0.0f;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
+      for (int s = 0; s < NS2; ++s) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if ((mask >> (i < 2 ? g : g + 8)) & 1u) tot[s][i] = fmaf(i < 2 ? w_lo : w_hi, acc[s][i], tot[s][i]);
@@ -590,64 +794,85 @@ __global__ void __launch_bounds__(kDecThreads, 2) moe_decode_kernel(const Decode
         }
       }
     };
-    int b = warp;
-    for (int slot = 0; slot < n_active; ++slot) {
-      if (b < nb2) {
-        const int e = sm.list[slot];
-        const uint32_t mask = sm.mask[e];
-        const bool use_lo = (mask >> g) & 1u, use_hi = (mask >> (g + 8)) & 1u;
-        int kb = b * 256 + t4 * 16;
-        const uint16_t* ap = p.act + (static_cast<int64_t>(slot) * p.M + g) * p.I + (b * 16 + t4) * ELT;
-        const int64_t a_hi = static_cast<int64_t>(8) * p.I;
-        const uint8_t* sp = p.s2 + (static_cast<int64_t>(e) * p.H + r0 + g) * sb2 + (WF == WF_NV4 ? kb >> 3 : kb >> 4);
-        const int64_t sb8 = static_cast<int64_t>(8) * sb2;
-        for (; b < nb2; b += kDecWarps) {
-          const uint8_t* at = nullptr;
-          if constexpr (WF == WF_16BIT) {
-            uint32_t lo[4][TR], hi[4][TR];
+    // the warp's steps in order: (slot, b), b + 8, ... on into the next slots
+    auto settle = [&](DecodeStep& s) {
+      while (s.b >= nb2 && s.slot < n_active) s.b -= nb2, ++s.slot;
+    };
+    auto operand = [&](const DecodeStep& s) {
+      return p.act + (static_cast<int64_t>(s.slot) * p.M + g) * p.I + (s.b * 8 * LN2 + t4) * ELT;
+    };
+    auto routed = [&](const DecodeStep& s, int row) { return ((sm.mask[sm.list[s.slot]] >> row) & 1u) != 0; };
+    const int64_t a_hi = static_cast<int64_t>(8) * p.I;
+    // The activations come from L2: those of the next step (4-bit: half step), whichever expert it belongs to, are
+    // requested before this one's are used.  (16-bit weights and more than 8 tokens: no registers left for that.)
+    constexpr bool AHEAD = WF != WF_16BIT || !HI;
+    DecodeStep cur{0, warp};
+    settle(cur);
+    if (AHEAD && cur.slot < n_active) {
+      const int kb = cur.b * (128 * LN2) + t4 * 16;
 #pragma unroll
-            for (int st = 0; st < 4; ++st) {
-              const bool in = kb + st * 64 < rb2;
-              load_tokens<BF16, WF>(ap + st * 4 * ELT, use_lo && in, true, lo[st]);
-              load_tokens<BF16, WF, HI>(ap + st * 4 * ELT + a_hi, use_hi && in, true, hi[st]);
-            }
-            at = next_stage();
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-              if (r0 + 8 * s < row1) {
-#pragma unroll
-                for (int st = 0; st < 4; ++st)
-                  chunk_mma<BF16, WF>(acc[s], chunk(at + s * 1024 + (st >> 1) * 2048, st & 1), 0, lo[st], hi[st]);
-              }
-          } else {
-#pragma unroll
-            for (int st = 0; st < 4; ++st) {
-              const bool in = kb + st * 64 < rb2;
-              uint32_t lo[TR], hi[TR], sc[2];
-              load_tokens<BF16, WF>(ap + st * 4 * ELT, use_lo && in, true, lo);
-              load_tokens<BF16, WF, HI>(ap + st * 4 * ELT + a_hi, use_hi && in, true, hi);
-#pragma unroll
-              for (int s = 0; s < 2; ++s) sc[s] = load_scales<WF>(sp + s * sb8 + st * SPB, r0 + 8 * s + g < row1 && in);
-              if (st == 0) at = next_stage();
-#pragma unroll
-              for (int s = 0; s < 2; ++s)
-                if (r0 + 8 * s < row1)
-                  chunk_mma<BF16, WF>(acc[s], chunk(at + s * 1024 + (st >> 1) * 2048, st & 1), sc[s], lo, hi);
-            }
-          }
-          __syncwarp();
-          issue();
-          kb += kDecWarps * 256;
-          ap += kDecWarps * 16 * ELT;
-          sp += kDecWarps * 4 * SPB;
-        }
-        fold(slot);
+      for (int st = 0; st < (WF == WF_16BIT ? 4 : 1); ++st) {
+        load_tokens<WF>(operand(cur) + st * 4 * ELT, routed(cur, g) && kb + st * 64 < rb2, lo[st]);
+        if constexpr (HI) load_tokens<WF>(operand(cur) + a_hi + st * 4 * ELT, routed(cur, g + 8) && kb + st * 64 < rb2, hi[st]);
       }
-      b -= nb2;
+    }
+    while (cur.slot < n_active) {
+      DecodeStep nxt{cur.slot, cur.b + kDecWarps};
+      settle(nxt);
+      const bool more = nxt.slot < n_active;
+      const int kb = cur.b * (128 * LN2) + t4 * 16, nkb = nxt.b * (128 * LN2) + t4 * 16;
+      if constexpr (WF == WF_16BIT) {
+        uint4 nlo[AHEAD ? 4 : 1][NV];
+        if constexpr (AHEAD) {
+          const uint16_t* np = more ? operand(nxt) : nullptr;
+          const bool use = more && routed(nxt, g);
+#pragma unroll
+          for (int st = 0; st < 4; ++st) {
+            nlo[st][0] = lo[st][0];
+            load_tokens<WF>(np + st * 4 * ELT, use && nkb + st * 64 < rb2, nlo[st]);
+          }
+        } else {
+          const uint16_t* ap = operand(cur);
+          const bool use_lo = routed(cur, g), use_hi = routed(cur, g + 8);
+#pragma unroll
+          for (int st = 0; st < 4; ++st) {
+            load_tokens<WF>(ap + st * 4 * ELT, use_lo && kb + st * 64 < rb2, lo[st]);
+            load_tokens<WF>(ap + st * 4 * ELT + a_hi, use_hi && kb + st * 64 < rb2, hi[st]);
+          }
+        }
+        const uint8_t *at, *no_scales;
+        next_stage(at, no_scales);
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+          for (int s = 0; s < NS2; ++s)
+            if (r0 + 8 * s < row1)
+              chunk_mma<BF16>(acc[s], chunk(at + s * 1024 + (st >> 1) * 2048, st & 1), lo[st][0], hi[st][0]);
+        if constexpr (AHEAD) {
+#pragma unroll
+          for (int st = 0; st < 4; ++st) lo[st][0] = nlo[st][0];
+        }
+      } else {
+        const uint16_t *ap = operand(cur), *nap = more ? operand(nxt) : ap;
+        const bool use_lo = routed(cur, g), use_hi = routed(cur, g + 8);
+        const bool nuse_lo = more && routed(nxt, g), nuse_hi = more && routed(nxt, g + 8);
+        auto fetch = [&](int st) {
+          constexpr int LAST = 2 * LN2 - 1;
+          const bool in = st < LAST ? kb + (st + 1) * 64 < rb2 : more && nkb < rb2;
+          const uint16_t* np = st < LAST ? ap + (st + 1) * 4 * ELT : nap;
+          load_tokens<WF>(np, (st < LAST ? use_lo : nuse_lo) && in, lo[(st & 1) ^ 1]);
+          if constexpr (HI) load_tokens<WF>(np + a_hi, (st < LAST ? use_hi : nuse_hi) && in, hi[(st & 1) ^ 1]);
+        };
+        full_step4<BF16, WF, NS2, LN2>(acc, lo, hi, fetch, next_stage);
+      }
+      __syncwarp();
+      issue();
+      if (nxt.slot != cur.slot) fold(cur.slot);
+      cur = nxt;
     }
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      float* o = sm.part[buf][warp] + (8 * s + 2 * t4) * PS + g;
+    for (int s = 0; s < NS2; ++s) {
+      float* o = sm.part[0][warp] + (8 * s + 2 * t4) * PS + g;
       o[0] = tot[s][0];
       o[PS] = tot[s][1];
       if constexpr (HI) {
@@ -656,19 +881,19 @@ __global__ void __launch_bounds__(kDecThreads, 2) moe_decode_kernel(const Decode
       }
     }
     __syncthreads();
-    {
-      const int r = threadIdx.x & 15, t = threadIdx.x >> 4;
-      if (t < p.M && r0 + r < row1) {
+    for (int i = threadIdx.x; i < 8 * NS2 * p.M; i += kDecThreads) {
+      const int r = i % (8 * NS2), t = i / (8 * NS2);
+      if (r0 + r < row1) {
         float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kDecWarps; ++w) v += sm.part[buf][w][r * PS + t];
+        for (int w = 0; w < kDecWarps; ++w) v += sm.part[0][w][r * PS + t];
         p.out[static_cast<int64_t>(t) * p.H + r0 + r] = static_cast<uint16_t>(pack2<BF16>(v, 0.0f));
       }
     }
-    if constexpr (Smem::kBufs == 2) buf ^= 1;
-    else __syncthreads();
+    __syncthreads();
   }
   cp_async_wait<0>();
+  decode_finish(p, base, epoch);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------
@@ -679,8 +904,9 @@ static DecodeWs decode_ws(int64_t M, int I, int E, int topk) {
   auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
   DecodeWs w;
   const int64_t active = M * topk < E ? M * topk : E;
-  w.logits = 256;                                                    // grid-barrier words first
-  w.act = w.logits + up(static_cast<size_t>(M) * E * sizeof(float));
+  w.logits = 256;                                                    // control words first
+  // the tagged logits always have the same place, so that no other call's data is ever taken for one
+  w.act = w.logits + static_cast<size_t>(kDecTokens) * kDecMaxExperts * sizeof(unsigned long long);
   w.total = w.act + up(static_cast<size_t>(active) * M * I * 2);
   return w;
 }
@@ -694,7 +920,7 @@ size_t moe_decode_workspace(int64_t M, int I, int E, int topk) {
 template <bool BF16, int WF, bool HI>
 static int launch_decode_rows(const DecodeParams& p, cudaStream_t st) {
   auto kern = moe_decode_kernel<BF16, WF, HI>;
-  constexpr int smem = sizeof(DecodeSmem<HI>);
+  constexpr int smem = sizeof(DecodeSmem<WF, HI>);
   // resident CTAs of the device, looked up once (0 = not yet)
   constexpr int kMaxDevices = 64;
   static std::atomic<int> grids[kMaxDevices];
@@ -706,13 +932,13 @@ static int launch_decode_rows(const DecodeParams& p, cudaStream_t st) {
     int per_sm = 0;
     FR_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kDecThreads, smem));
     if (per_sm < 1) return FR_ERR_UNSUPPORTED;
-    grid = (per_sm > 2 ? 2 : per_sm) * di.sm_count;
+    grid = std::min(per_sm, DecodeCfg<WF, HI>::TWO ? 2 : 1) * di.sm_count;
     grids[di.device].store(grid, std::memory_order_release);
   }
   DecodeParams q = p;
-  // one (expert, group of tokens) per CTA where the grid is large enough
-  q.tokens_per_unit = static_cast<int>((static_cast<int64_t>(p.M) * p.E + grid - 1) / grid);
-  if (q.tokens_per_unit > p.M) q.tokens_per_unit = p.M;
+  // router: as many groups of tokens per expert as leave every CTA at most one (expert, group)
+  const int groups = std::max(1, std::min(p.M, grid / p.E));
+  q.tokens_per_unit = (p.M + groups - 1) / groups;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kDecThreads);
@@ -772,11 +998,18 @@ int moe_decode_dispatch(const void* x, const void* gate, int64_t gsh, int64_t gs
   p.topk = topk;
   p.renormalize = renormalize;
   p.tokens_per_unit = 1;
+  // the largest copy that every row's start allows (a step's scales are 16 bytes, or 8 for blocks of 32)
+  auto scale_copy = [&](const void* s, int k) {
+    const uintptr_t u = reinterpret_cast<uintptr_t>(s) | static_cast<uintptr_t>(k / (block ? block : 1));
+    return block == 0 ? 0 : (block == 16 && !(u & 15)) ? 16 : !(u & 7) ? 8 : !(u & 3) ? 4 : 0;
+  };
+  p.scale_copy1 = scale_copy(s1, H);
+  p.scale_copy2 = scale_copy(s2, I);
   p.out = static_cast<uint16_t*>(out);
   p.tw = tw;
   p.ti = ti;
-  p.barrier = reinterpret_cast<unsigned int*>(base);
-  p.logits = reinterpret_cast<float*>(base + ws.logits);
+  p.control = reinterpret_cast<unsigned int*>(base);
+  p.logits = reinterpret_cast<unsigned long long*>(base + ws.logits);
   p.act = reinterpret_cast<uint16_t*>(base + ws.act);
   const bool bf = dtype == FR_BF16;
   if (block == 0) return bf ? launch_decode<true, WF_16BIT>(p, st) : launch_decode<false, WF_16BIT>(p, st);
