@@ -1495,7 +1495,7 @@ int fr_fp4_gemm(const void* a_q, const void* a_scale, const float* a_global, con
 }
 
 size_t fr_moe_decode_workspace_bytes(int64_t M, int H, int I, int E, int topk) {
-  return H > 0 ? fr::moe_decode_workspace(M, I, E, topk) : 0;
+  return fr::moe_decode_workspace(M, H, I, E, topk);
 }
 
 int fr_moe_decode(const void* x, const void* gate, int64_t gate_stride_h, int64_t gate_stride_e, const void* w1,

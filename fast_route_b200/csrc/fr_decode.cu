@@ -37,7 +37,8 @@ constexpr int kDecScaleBytes = 512;                // and, for 4-bit weights, 32
 
 // Control words of a workspace: zero before the first call, kept up by every call (the CTA that finishes last adds what
 // the call used, so nothing has to be cleared in between).
-enum { DC_COUNT = 0, DC_BASE = 1, DC_FINISHED = 2, DC_BUDGET = 3, DC_EPOCH = 4 };
+enum { DC_COUNT = 0, DC_BASE = 1, DC_FINISHED = 2, DC_BUDGET = 3, DC_EPOCH = 4, DC_GROUP = 64 /* one per row range */ };
+constexpr int kDecMaxGroups = 512;
 constexpr uint32_t kDecPolls = 1u << 22;           // about a second, unless DC_BUDGET holds another limit
 
 enum { WF_16BIT = 0, WF_NV4 = 1, WF_MX4 = 2 };
@@ -52,6 +53,8 @@ struct DecodeParams {
   const float *g1, *g2;          // one fp32 scale per expert, or null
   int M, H, I, E, topk, renormalize;
   int scale_copy1, scale_copy2;  // bytes per cp.async of w1's / w2's scales: 16, 8 or 4; 0: rows start anywhere
+  int ksplit, groups;            // GEMM2: `groups` row ranges, each shared by `ksplit` CTAs that split K
+  float* partial;                // [ksplit][M][H], with ksplit > 1
   int tokens_per_unit;           // router: tokens one CTA takes for one expert
   uint16_t* out;
   float* tw;
@@ -78,12 +81,12 @@ struct DecodeSmem {
   using C = DecodeCfg<WF, HI>;
   uint8_t ring[kDecWarps][C::STAGES][C::STAGE];
   float part[C::PBUFS][kDecWarps][32 * C::STRIDE];
-  float weight[kDecMaxExperts][C::TOKENS];    // routing weight by slot (position in `list`) and token
-  uint32_t mask[kDecMaxExperts];              // by expert: bit t = token t goes there; upper half: its slot
+  float weight[kDecMaxExperts][C::TOKENS];    // routing weight by expert and token
+  uint32_t mask[kDecMaxExperts];              // by expert: bit t = token t goes there
   uint16_t list[kDecMaxExperts];              // active experts in ascending order
   uint32_t scan[kDecWarps];
   uint32_t base, epoch;                       // of the control words, read once
-  int ok;
+  int ok, last;
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t size) {
@@ -341,9 +344,9 @@ __device__ __forceinline__ uint32_t order_key(float v) {   // larger value, larg
 // Every CTA ranks all tokens: a warp polls the logits of its (up to two) tokens until all carry this call's tag
 // (bounded), then k rounds of arg-max (equal logits: lower expert id), softmax by the fixed fp32 recipe of the routers.
 // `sel` / `val`: [kDecTokens][E] scratch.  False: the logits did not arrive in time.
-template <class Smem, int NT>
+// NE: logits per lane, NT: tokens per warp.
+template <int NE, int NT, class Smem>
 __device__ __forceinline__ bool decode_rank(const DecodeParams& p, Smem& sm, uint32_t tag, uint16_t* sel, float* val) {
-  constexpr int NE = kDecMaxExperts / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int e = threadIdx.x; e < p.E; e += kDecThreads) sm.mask[e] = 0;
   __syncthreads();
@@ -360,7 +363,7 @@ __device__ __forceinline__ bool decode_rank(const DecodeParams& p, Smem& sm, uin
         for (int i = 0; i < NE; ++i) {
           const int t = warp + n * kDecWarps, c = i * 32 + lane;
           u[n][i] = static_cast<unsigned long long>(tag) << 32;
-          if (i * 32 < p.E && t < p.M && c < p.E)
+          if (t < p.M && c < p.E)
             asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(u[n][i]) : "l"(p.logits + static_cast<int64_t>(t) * p.E + c));
         }
       bool mine = true;
@@ -373,6 +376,7 @@ __device__ __forceinline__ bool decode_rank(const DecodeParams& p, Smem& sm, uin
           key[n][i] = i * 32 + lane < p.E ? order_key(v[n][i]) : 0u;
         }
       all = __all_sync(0xffffffffu, mine);
+      if (!all) __nanosleep(300);      // every CTA polls the same lines: without a pause the stores wait for the polls
     }
     if (!all && lane == 0) {
       report(ST_WAIT_TIMEOUT, 0x800);
@@ -387,7 +391,7 @@ __device__ __forceinline__ bool decode_rank(const DecodeParams& p, Smem& sm, uin
         float bv = 0.0f;
 #pragma unroll
         for (int i = 0; i < NE; ++i)
-          if (i * 32 < p.E && key[n][i] > best) best = key[n][i], at = i, bv = v[n][i];
+          if (key[n][i] > best) best = key[n][i], at = i, bv = v[n][i];
         const uint32_t top = __reduce_max_sync(0xffffffffu, best);
         const uint32_t col = __reduce_min_sync(0xffffffffu, best == top ? static_cast<uint32_t>(at * 32 + lane) : 0xFFFFu);
         if (t < p.M && col == static_cast<uint32_t>(at * 32 + lane)) {
@@ -424,7 +428,7 @@ __device__ __forceinline__ bool decode_rank(const DecodeParams& p, Smem& sm, uin
       __syncwarp();
       for (int j = lane; j < p.topk; j += 32) {
         const float w = __fdiv_rn(my_val[j], s);
-        my_val[j] = w;
+        sm.weight[sel[t * p.E + j]][t] = w;
         if (blockIdx.x == 0 && p.tw) {
           p.tw[static_cast<int64_t>(t) * p.topk + j] = w;
           p.ti[static_cast<int64_t>(t) * p.topk + j] = sel[t * p.E + j];
@@ -441,17 +445,7 @@ __device__ __forceinline__ bool decode_rank(const DecodeParams& p, Smem& sm, uin
   __syncthreads();
   uint32_t before = 0;
   for (int w = 0; w < warp; ++w) before += sm.scan[w];
-  const uint32_t slot = before + __popc(vote & ((1u << lane) - 1u));
-  // the slot of an expert, in the upper half of its mask word
-  if (active) {
-    sm.list[slot] = static_cast<uint16_t>(threadIdx.x);
-    sm.mask[threadIdx.x] |= slot << 16;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < p.M * p.topk; i += kDecThreads) {
-    const int t = i / p.topk, j = i - t * p.topk;
-    sm.weight[sm.mask[sel[t * p.E + j]] >> 16][t] = val[t * p.E + j];
-  }
+  if (active) sm.list[before + __popc(vote & ((1u << lane) - 1u))] = static_cast<uint16_t>(threadIdx.x);
   __syncthreads();
   return true;
 }
@@ -486,8 +480,11 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
   __syncthreads();
   const uint32_t base = sm.base, epoch = sm.epoch;
   decode_logits<BF16>(p, epoch + 1, &sm.part[0][0][0]);
-  if (!decode_rank<Smem, HI ? 2 : 1>(p, sm, epoch + 1, reinterpret_cast<uint16_t*>(&sm.part[0][0][0]),
-                   reinterpret_cast<float*>(&sm.ring[0][0][0]))) {
+  uint16_t* sel = reinterpret_cast<uint16_t*>(&sm.part[0][0][0]);
+  float* val = reinterpret_cast<float*>(&sm.ring[0][0][0]);
+  constexpr int NT = HI ? 2 : 1;
+  if (!(p.E <= 64 ? decode_rank<2, NT>(p, sm, epoch + 1, sel, val)
+                  : decode_rank<kDecMaxExperts / 32, NT>(p, sm, epoch + 1, sel, val))) {
     if (threadIdx.x == 0) atomicAdd(p.control + DC_COUNT, 1u);      // the others' barrier counts every CTA
     decode_finish(p, base, epoch);
     return;
@@ -501,11 +498,15 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
   const int sb1 = WF == WF_NV4 ? p.H / 16 : p.H / 32;   // scale bytes of a row
   const int sb2 = WF == WF_NV4 ? p.I / 16 : p.I / 32;
 
-  // this CTA's share: row pairs [pair0, pair1) of the active experts' w1, rows [row0, row1) of every active w2
+  // this CTA's share: row pairs [pair0, pair1) of the active experts' w1, rows [row0, row1) of every active w2, of which
+  // it takes every ksplit-th part of K
   const int64_t pairs = static_cast<int64_t>(n_active) * p.I;
   const int64_t pair0 = pairs * blockIdx.x / G, pair1 = pairs * (blockIdx.x + 1) / G;
-  const int row0 = static_cast<int>(static_cast<int64_t>(p.H) * blockIdx.x / G);
-  const int row1 = static_cast<int>(static_cast<int64_t>(p.H) * (blockIdx.x + 1) / G);
+  const int ks = static_cast<int>(blockIdx.x) / p.groups, group = static_cast<int>(blockIdx.x) - ks * p.groups;
+  const bool second = ks < p.ksplit;                   // the last few CTAs may have no part in GEMM2
+  const int row0 = second ? static_cast<int>(static_cast<int64_t>(p.H) * group / p.groups) : 0;
+  const int row1 = second ? static_cast<int>(static_cast<int64_t>(p.H) * (group + 1) / p.groups) : 0;
+  const int w2nd = ks * kDecWarps + warp, n2nd = p.ksplit * kDecWarps;     // this warp among those of its rows
 
   // A step is 128 bytes (a full line) of every row of a tile.  GEMM1: tiles of 16 pairs = four sub-tiles of 4 SiLU + 4
   // linear rows, warp w takes steps w, w + 8, ...; GEMM2: tiles of 16 rows = two sub-tiles of 8, two steps at a time,
@@ -520,7 +521,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
   const int cr = lane >> 3, cc = lane & 7;
   int64_t ld_left = pair1 - pair0;     // GEMM1 pairs from the next segment on
   int ld_a = static_cast<int>(pair0 / p.I), ld_j = static_cast<int>(pair0 - static_cast<int64_t>(ld_a) * p.I);
-  int ld_row = row0, ld_slot = 0, ld_b2 = warp;
+  int ld_row = row0, ld_slot = 0, ld_b2 = w2nd;
   int ld_rem = 0, ld_k = 0, ld_rows = 0;
   bool ld_second = false;
   const uint8_t* ld_src = p.w1;
@@ -560,17 +561,17 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
         ld_k = ld_b2 * (128 * LN2) + cc * 16;
         ld_src = p.w2 + row * rb2 + ld_k;
         ld_rows = row1 - ld_row - cr;
-        if (ld_b2 < nb2) ld_rem = (nb2 - ld_b2 + kDecWarps - 1) / kDecWarps;
+        if (ld_b2 < nb2) ld_rem = (nb2 - ld_b2 + n2nd - 1) / n2nd;
         if constexpr (WF != WF_16BIT) {
           const int off = (ld_b2 * 2 + (lane >> 4)) * SCB;
           ld_sc_ok = ld_row + (lane & 15) < row1;
           ld_sc_left = sb2 - off;
           ld_sc = p.s2 + (static_cast<int64_t>(sm.list[ld_slot]) * p.H + ld_row + (lane & 15)) * sb2 + off;
         }
-        ld_b2 += ld_rem * kDecWarps - nb2;
+        ld_b2 += ld_rem * n2nd - nb2;
         if (++ld_slot == n_active) {
           ld_slot = 0;
-          ld_b2 = warp;
+          ld_b2 = w2nd;
           ld_row += 8 * NS2;
         }
       } else {
@@ -610,12 +611,12 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
         }
         src += step;
       }
-      ld_k += kDecWarps * 128 * LN2;
-      ld_src += kDecWarps * 128 * LN2;
+      ld_k += n2nd * 128 * LN2;
+      ld_src += n2nd * 128 * LN2;
       if constexpr (WF != WF_16BIT) {
         if (ld_sc_ok) cp_async_scales<SCB>(sc_ring + ld_at, ld_sc_left > 0 ? ld_sc : p.s2, ld_sc_left, p.scale_copy2);
-        ld_sc += kDecWarps * 2 * SCB;
-        ld_sc_left -= kDecWarps * 2 * SCB;
+        ld_sc += n2nd * 2 * SCB;
+        ld_sc_left -= n2nd * 2 * SCB;
       }
     }
     --ld_rem;
@@ -784,7 +785,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
       const uint32_t mask = sm.mask[e];
       float f = 1.0f;
       if constexpr (WF != WF_16BIT) f = (p.g2 ? __ldg(p.g2 + e) : 1.0f) * Fp4Expand<BF16, WF>::kUnit;
-      const float w_lo = sm.weight[from][g] * f, w_hi = HI ? sm.weight[from][(g + 8) % C::TOKENS] * f : 0.0f;
+      const float w_lo = sm.weight[e][g] * f, w_hi = HI ? sm.weight[e][(g + 8) % C::TOKENS] * f : 0.0f;
 #pragma unroll
       for (int s = 0; s < NS2; ++s) {
 #pragma unroll
@@ -794,7 +795,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
         }
       }
     };
-    // the warp's steps in order: (slot, b), b + 8, ... on into the next slots
+    // the warp's steps in order: (slot, b), then every n2nd-th, on into the next slots
     auto settle = [&](DecodeStep& s) {
       while (s.b >= nb2 && s.slot < n_active) s.b -= nb2, ++s.slot;
     };
@@ -806,7 +807,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
     // The activations come from L2: those of the next step (4-bit: half step), whichever expert it belongs to, are
     // requested before this one's are used.  (16-bit weights and more than 8 tokens: no registers left for that.)
     constexpr bool AHEAD = WF != WF_16BIT || !HI;
-    DecodeStep cur{0, warp};
+    DecodeStep cur{0, w2nd};
     settle(cur);
     if (AHEAD && cur.slot < n_active) {
       const int kb = cur.b * (128 * LN2) + t4 * 16;
@@ -817,7 +818,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
       }
     }
     while (cur.slot < n_active) {
-      DecodeStep nxt{cur.slot, cur.b + kDecWarps};
+      DecodeStep nxt{cur.slot, cur.b + n2nd};
       settle(nxt);
       const bool more = nxt.slot < n_active;
       const int kb = cur.b * (128 * LN2) + t4 * 16, nkb = nxt.b * (128 * LN2) + t4 * 16;
@@ -887,33 +888,62 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
         float v = 0.0f;
 #pragma unroll
         for (int w = 0; w < kDecWarps; ++w) v += sm.part[0][w][r * PS + t];
-        p.out[static_cast<int64_t>(t) * p.H + r0 + r] = static_cast<uint16_t>(pack2<BF16>(v, 0.0f));
+        const int64_t at = static_cast<int64_t>(t) * p.H + r0 + r;
+        if (p.ksplit == 1) p.out[at] = static_cast<uint16_t>(pack2<BF16>(v, 0.0f));
+        else __stcg(p.partial + static_cast<int64_t>(ks) * p.M * p.H + at, v);
       }
     }
     __syncthreads();
   }
   cp_async_wait<0>();
+  if (p.ksplit > 1 && second) {
+    // whoever comes last of the CTAs that share these rows adds their sums, in the order of their shares of K
+    if (threadIdx.x == 0) {
+      __threadfence();
+      sm.last = atomicAdd(p.control + DC_GROUP + group, 1u) == static_cast<unsigned int>(p.ksplit) - 1u;
+      __threadfence();
+    }
+    __syncthreads();
+    if (sm.last) {
+      const int rows = row1 - row0;
+      for (int i = threadIdx.x; i < rows * p.M; i += kDecThreads) {
+        const int64_t at = static_cast<int64_t>(i / rows) * p.H + row0 + i % rows;
+        float v = 0.0f;
+        for (int s = 0; s < p.ksplit; ++s) v += __ldcg(p.partial + static_cast<int64_t>(s) * p.M * p.H + at);
+        p.out[at] = static_cast<uint16_t>(pack2<BF16>(v, 0.0f));
+      }
+      if (threadIdx.x == 0) p.control[DC_GROUP + group] = 0;
+    }
+  }
   decode_finish(p, base, epoch);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------
+// GEMM2: CTAs per row range, so that a range has about 14 rows.  With fewer the warps' steps hold few bytes and their
+// number (active experts * I / 8 warps) times the latency of one is what the product takes: 16 tokens, 64 experts,
+// H = I = 512, 1.7 rows per CTA: 68 us, with eight CTAs per range 47.
+static int decode_ksplit(int grid, int H) {
+  const int k = (grid * 14 + H / 2) / H;
+  return k < 1 ? 1 : (k > 16 ? 16 : k);
+}
 struct DecodeWs {
-  size_t logits, act, total;
+  size_t logits, partial, act, total;
 };
-static DecodeWs decode_ws(int64_t M, int I, int E, int topk) {
+static DecodeWs decode_ws(int64_t M, int H, int I, int E, int topk) {
   auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
   DecodeWs w;
   const int64_t active = M * topk < E ? M * topk : E;
-  w.logits = 256;                                                    // control words first
+  w.logits = up((DC_GROUP + kDecMaxGroups) * sizeof(unsigned int));  // control words first
   // the tagged logits always have the same place, so that no other call's data is ever taken for one
-  w.act = w.logits + static_cast<size_t>(kDecTokens) * kDecMaxExperts * sizeof(unsigned long long);
+  w.partial = w.logits + static_cast<size_t>(kDecTokens) * kDecMaxExperts * sizeof(unsigned long long);
+  w.act = w.partial + up(static_cast<size_t>(M) * (14 * kDecMaxGroups + H) * sizeof(float));   // ksplit * H of them each
   w.total = w.act + up(static_cast<size_t>(active) * M * I * 2);
   return w;
 }
 
-size_t moe_decode_workspace(int64_t M, int I, int E, int topk) {
-  if (M <= 0 || M > kDecTokens || I <= 0 || E <= 0 || topk <= 0 || topk > E) return 0;
-  return decode_ws(M, I, E, topk).total;
+size_t moe_decode_workspace(int64_t M, int H, int I, int E, int topk) {
+  if (M <= 0 || M > kDecTokens || H <= 0 || I <= 0 || E <= 0 || topk <= 0 || topk > E) return 0;
+  return decode_ws(M, H, I, E, topk).total;
 }
 
 // HI: more than 8 tokens, the second half of the MMA's row side is used
@@ -936,6 +966,9 @@ static int launch_decode_rows(const DecodeParams& p, cudaStream_t st) {
     grids[di.device].store(grid, std::memory_order_release);
   }
   DecodeParams q = p;
+  q.ksplit = decode_ksplit(grid, p.H);
+  q.groups = grid / q.ksplit;
+  if (grid > kDecMaxGroups) return FR_ERR_UNSUPPORTED;
   // router: as many groups of tokens per expert as leave every CTA at most one (expert, group)
   const int groups = std::max(1, std::min(p.M, grid / p.E));
   q.tokens_per_unit = (p.M + groups - 1) / groups;
@@ -966,7 +999,7 @@ int moe_decode_dispatch(const void* x, const void* gate, int64_t gsh, int64_t gs
   if (block != 0 && block != 16 && block != 32) return FR_ERR_ARG;
   if ((tw == nullptr) != (ti == nullptr)) return FR_ERR_ARG;
   if (dtype != FR_F16 && dtype != FR_BF16) return FR_ERR_UNSUPPORTED;
-  if (M > kDecTokens || E > kDecMaxExperts) return FR_ERR_UNSUPPORTED;
+  if (M > kDecTokens || E > kDecMaxExperts || H > (1 << 22) || I > (1 << 22)) return FR_ERR_UNSUPPORTED;
   if (block == 32 && dtype != FR_BF16) return FR_ERR_UNSUPPORTED;     // E8M0 scales reach beyond fp16
   const int unit = block ? 32 : 8;                                    // 16 bytes of a weight row
   if (H % unit || I % unit) return FR_ERR_ALIGN;
@@ -975,7 +1008,7 @@ int moe_decode_dispatch(const void* x, const void* gate, int64_t gsh, int64_t gs
   for (const void* q : {x, w1, w2})
     if (reinterpret_cast<uintptr_t>(q) & 15) return FR_ERR_ALIGN;
   if (block == 16 && ((reinterpret_cast<uintptr_t>(s1) | reinterpret_cast<uintptr_t>(s2)) & 1)) return FR_ERR_ALIGN;
-  const DecodeWs ws = decode_ws(M, I, E, topk);
+  const DecodeWs ws = decode_ws(M, H, I, E, topk);
   if (!workspace || workspace_bytes < ws.total) return FR_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 255) return FR_ERR_ALIGN;
   uint8_t* base = static_cast<uint8_t*>(workspace);
@@ -1010,6 +1043,7 @@ int moe_decode_dispatch(const void* x, const void* gate, int64_t gsh, int64_t gs
   p.ti = ti;
   p.control = reinterpret_cast<unsigned int*>(base);
   p.logits = reinterpret_cast<unsigned long long*>(base + ws.logits);
+  p.partial = reinterpret_cast<float*>(base + ws.partial);
   p.act = reinterpret_cast<uint16_t*>(base + ws.act);
   const bool bf = dtype == FR_BF16;
   if (block == 0) return bf ? launch_decode<true, WF_16BIT>(p, st) : launch_decode<false, WF_16BIT>(p, st);
