@@ -1007,7 +1007,6 @@ int moe_decode_dispatch(const void* x, const void* gate, int64_t gsh, int64_t gs
   if (!x || !gate || !w1 || !w2 || !out || (block && (!s1 || !s2))) return FR_ERR_ARG;
   for (const void* q : {x, w1, w2})
     if (reinterpret_cast<uintptr_t>(q) & 15) return FR_ERR_ALIGN;
-  if (block == 16 && ((reinterpret_cast<uintptr_t>(s1) | reinterpret_cast<uintptr_t>(s2)) & 1)) return FR_ERR_ALIGN;
   const DecodeWs ws = decode_ws(M, H, I, E, topk);
   if (!workspace || workspace_bytes < ws.total) return FR_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 255) return FR_ERR_ALIGN;

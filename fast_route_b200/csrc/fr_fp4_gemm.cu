@@ -11,9 +11,10 @@
 //
 // The scales lie row by row in global memory; the hardware wants, for 128 rows, 512-byte blocks of 32 rows x 4 row
 // groups x 4 bytes.  For more than 128 tokens a small kernel lays them out that way in the workspace first (6 MB for
-// 8192 x 14336 x 4096) and the producer fetches 2 KB blocks; loading them row by row inside the product, with at most
-// four stages of look-ahead, took four times the MMAs' own time (684 us instead of 185).  Up to 128 tokens a second
-// launch would cost more than it saves: four loader warps put each 4-byte group in its place with cp.async.
+// 8192 x 14336 x 4096) and the producer fetches 2 KB blocks: loading them row by row inside the product asks for 4 bytes
+// of 32 different lines per instruction (684 us instead of 300).  Up to 128 tokens four loader warps do just that with
+// cp.async: the second launch costs as much as it saves (128 x 14336 x 4096: 25 us either way, 17 of them the product
+// when the scales are laid out; 100 x 4096 x 4096: 13.6 against 16.8).
 //
 // Every stage has its own columns in tensor memory for its scales, so a copy never overwrites scales that an MMA in
 // flight may still read: the stage is refilled only after its MMAs have completed.
@@ -273,8 +274,8 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   } else if (warp < C::EPI0) {
     if constexpr (!C::LAID) {
     // ------------------------------ scale loaders -----------------------------
-    // Thread r copies the scales of lane row r and of column rows r (and 128 + r).  The copies of two stages are in
-    // flight behind the one being handed over.
+    // Thread r copies the scales of lane row r and of column row r.  The copies of two stages are in flight behind
+    // the one being handed over.
     constexpr int LOOK = 2, SB = FG_KSTAGE / BLOCK, W = SB / 4;
     const int r = (warp - 2) * 32 + lane;
     const bool aligned = (p.spitch & 3) == 0 && ((reinterpret_cast<uintptr_t>(p.sa) | reinterpret_cast<uintptr_t>(p.sb)) & 3) == 0;
@@ -543,10 +544,10 @@ static FgPlan fp4_plan(int64_t m, int64_t n, int64_t k, int block) {
   q.tiles_a = static_cast<int>((ra + FG_LANES - 1) / FG_LANES);
   q.tiles_b = static_cast<int>((rb + q.bn - 1) / q.bn);
   q.groups_a = q.tiles_a;
-  q.groups_b = q.tiles_b * (q.bn / 128);
+  q.groups_b = q.bn < 256 ? 0 : q.tiles_b * (q.bn / 128);       // 0: no layout pass
   q.sblk = block == 16 ? 2048 : 1024;
   q.ws_a = static_cast<size_t>(q.groups_a) * q.kstages * q.sblk;
-  q.ws_total = q.swapped ? 0 : q.ws_a + static_cast<size_t>(q.groups_b) * q.kstages * q.sblk;
+  q.ws_total = q.groups_b ? q.ws_a + static_cast<size_t>(q.groups_b) * q.kstages * q.sblk : 0;
   return q;
 }
 static bool fp4_gemm_sizes_ok(int64_t m, int64_t n, int64_t k) {
@@ -594,7 +595,7 @@ int fp4_gemm_dispatch(const void* a_q, const void* a_scale, const float* a_globa
   if (rc) return rc;
   rc = make_tmap_2d(&mb, q.swapped ? a_q : b_q, p.rows_b, kb, kb, q.bn, 128, true, 1);
   if (rc) return rc;
-  if (!q.swapped) {
+  if (q.groups_b) {
     FgLayout l;
     l.sa = p.sa;
     l.sb = p.sb;
@@ -614,11 +615,13 @@ int fp4_gemm_dispatch(const void* a_q, const void* a_scale, const float* a_globa
     p.sa = l.da;
     p.sb = l.db;
   }
-  // split K while the tiles leave at least half of the SMs idle and every CTA keeps a stage
+  // Split K while the tiles leave at least half of the SMs idle, every CTA keeps a stage, and all clusters run at once: a
+  // cluster sits in one GPC, so eight CTAs of a whole SM each fit 16 times at most, four 32 times (333 x 1399 x 2080,
+  // 18 tiles: 24.8 us with eight, in two waves).
   const DeviceInfo& di = device_info();
   const int64_t tiles = static_cast<int64_t>(q.tiles_a) * q.tiles_b;
   int split = 1;
-  while (split < 8 && tiles * split * 2 <= di.sm_count && split * 2 <= p.kstages) split *= 2;
+  while (split < 8 && tiles * split * 2 <= di.sm_count && split * 2 <= p.kstages && tiles * split * 2 <= 128) split *= 2;
   p.split = split;
   const int grid = split > 1 ? static_cast<int>(tiles * split) : static_cast<int>(tiles < di.sm_count ? tiles : di.sm_count);
   const bool bf = dtype == FR_BF16;

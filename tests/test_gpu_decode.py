@@ -254,6 +254,78 @@ def test_graphs_and_streams(dev):
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(eager, want[2])
 
 
+@pytest.mark.reads_status
+def test_a_wait_that_runs_out_is_reported(dev):
+    """The wait for the other CTAs' activations is bounded: with the barrier's base moved up by one it can never be
+    satisfied, so it ends after the poll budget written into the control words, and the status block says so.  A zeroed
+    workspace serves the next call."""
+    from fast_route_b200 import _lib
+    M, H, I, E, k = 2, 256, 128, 4, 2
+    x, gate, w1, w2 = (t.to(dev) for t in synth.moe_inputs(M, H, I, E, seed=2, dtype=torch.bfloat16))
+    lib = _lib.load()
+    nbytes = lib.fr_moe_decode_workspace_bytes(M, H, I, E, k)
+    ws = torch.zeros(nbytes + 1024, dtype=torch.uint8, device=dev)
+    ws = ws[(-ws.data_ptr()) % 1024:][:nbytes]
+    out = torch.empty_like(x)
+
+    def call():
+        return lib.fr_moe_decode(_lib.ptr(x), _lib.ptr(gate), gate.stride(0), gate.stride(1), _lib.ptr(w1), None, None,
+                                 _lib.ptr(w2), None, None, 1, 0, M, H, I, E, k, 1, _lib.ptr(out), None, None, _lib.ptr(ws),
+                                 nbytes, _lib.stream_ptr(dev))
+    assert call() == 0
+    torch.cuda.synchronize()
+    assert _lib.device_status()[0] == 0
+    want = out.clone()
+    words = ws[:32].view(torch.int32)
+    assert int(words[0]) == int(words[1]) > 0 and int(words[2]) == 0 and int(words[4]) == 1
+    words[1] += 1                              # base
+    words[3] = 2000                            # polls
+    assert call() == 0
+    torch.cuda.synchronize()
+    code, detail, _, count = _lib.device_status()
+    assert code == 1 and detail == 0x802 and count > 0
+    ws.zero_()
+    assert call() == 0
+    torch.cuda.synchronize()
+    assert _lib.device_status()[0] == 0 and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("block,dt", [(16, torch.bfloat16), (32, torch.bfloat16)])
+@pytest.mark.parametrize("H,I", [(32, 32), (96, 160), (544, 224), (64, 2080)])
+def test_scales_that_start_anywhere(dev, H, I, block, dt):
+    """Row lengths and tensor offsets that leave the scale rows without any alignment, equal to the aligned result."""
+    M, E, k = 5, 3, 2
+    x, gate, w1, w2 = (t.to(dev) for t in synth.moe_inputs(M, H, I, E, seed=H + I, dtype=dt, weight_std=0.05))
+    q1, s1, g1, q2, s2, g2 = fr.quantize_experts_fp4(w1, w2, block)
+    want = fr.fused_moe_decode_fp4(x, gate, q1, s1, q2, s2, k, w1_global=g1, w2_global=g2)
+    for off in (1, 2, 3, 4, 8):
+        moved = []
+        for s in (s1, s2):
+            buf = torch.zeros(s.numel() + 16, dtype=torch.uint8, device=dev)
+            buf[off:off + s.numel()] = s.view(torch.uint8).flatten()
+            moved.append(buf[off:off + s.numel()].view(s.dtype).view(s.shape))
+        assert torch.equal(fr.fused_moe_decode_fp4(x, gate, q1, moved[0], q2, moved[1], k, w1_global=g1, w2_global=g2), want)
+
+
+def test_many_calls_of_changing_size_share_one_workspace(dev):
+    """Sizes, formats and numbers of tokens in turn on one stream: what one call leaves behind never reaches the next."""
+    cases = []
+    for i, (M, H, I, E, k) in enumerate([(1, 256, 512, 4, 2), (16, 512, 96, 32, 6), (3, 2048, 64, 8, 1), (9, 64, 1024, 200, 4),
+                                         (16, 1024, 256, 8, 8), (2, 4096, 32, 3, 2)]):
+        x, gate, w1, w2 = (t.to(dev) for t in synth.moe_inputs(M, H, I, E, seed=i, dtype=torch.bfloat16, weight_std=0.05))
+        cases.append((x, gate, w1, w2, k, fr.quantize_experts_fp4(w1, w2)))
+
+    def go(c):
+        x, gate, w1, w2, k, q = c
+        return (fr.fused_moe_decode(x, gate, w1, w2, k),
+                fr.fused_moe_decode_fp4(x, gate, q[0], q[1], q[3], q[4], k, w1_global=q[2], w2_global=q[5]))
+    want = [go(c) for c in cases]
+    order = np.random.default_rng(0).integers(0, len(cases), 60)
+    got = [(i, go(cases[i])) for i in order]
+    for i, (a, b) in got:
+        assert torch.equal(a, want[i][0]) and torch.equal(b, want[i][1])
+
+
 def test_decode_and_prompt_through_the_same_quantised_experts(dev):
     """As a server uses them together: experts quantised once, the prompt through fused_moe on the expanded weights (exact
     in bf16 but for the rounding of the global scale), the following tokens through the few-token layer."""

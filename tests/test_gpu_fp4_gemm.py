@@ -127,6 +127,23 @@ def test_quantise_then_multiply(dev):
         assert rel < 0.25
 
 
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("m", [9, 70, 200])
+def test_scales_that_start_anywhere(dev, block, m):
+    g = torch.Generator().manual_seed(10)
+    n, k = 140, 608                                     # scale rows of 38 or 19 bytes
+    a, b = _matrix(g, block, m, k), _matrix(g, block, n, k)
+    (aq, asc, _), (bq, bsc, _) = _dev(a, dev), _dev(b, dev)
+    want = fr.matmul_fp4(aq, asc, bq, bsc)
+    for off in (1, 2, 4):
+        moved = []
+        for s in (asc, bsc):
+            buf = torch.zeros(s.numel() + 16, dtype=torch.uint8, device=dev)
+            buf[off:off + s.numel()] = s.view(torch.uint8).flatten()
+            moved.append(buf[off:off + s.numel()].view(s.dtype).view(s.shape))
+        assert torch.equal(fr.matmul_fp4(aq, moved[0], bq, moved[1]), want)
+
+
 def test_empty_and_refusals(dev):
     g = torch.Generator().manual_seed(8)
     aq, asc, ag = _dev(_matrix(g, 16, 6, 64), dev)
