@@ -9,7 +9,6 @@ from __future__ import annotations
 
 import ctypes
 import os
-from contextlib import nullcontext
 from ctypes import c_char_p, c_int, c_int64, c_size_t, c_void_p
 
 import torch
@@ -133,11 +132,9 @@ def require_device(device, *tensors) -> None:
             raise FastRouteError(f"tensors on different devices: {t.device} and {device}")
 
 
-def on_device(device):
-    """Makes ``device`` the current one for a call (kernels launch on the current device)."""
-    if torch.cuda.current_device() == device.index:
-        return nullcontext()
-    return torch.cuda.device(device)
+def elsewhere(device) -> bool:
+    """Whether ``device`` is not the current one (kernels launch on the current device)."""
+    return torch.cuda.current_device() != device.index
 
 
 def device_status():

@@ -22,22 +22,25 @@ def _run(hidden_states, gate, w1, w2, dims, topk, renormalize, inplace, return_r
     assert M <= MAX_TOKENS, f"{M} tokens: at most {MAX_TOKENS}; use fused_moe for larger batches"
     dev = hidden_states.device
     _lib.require_device(dev, gate, w1, w2, s1, g1, s2, g2)
-    with _lib.on_device(dev):
-        out = hidden_states if inplace else torch.empty_like(hidden_states)
-        tw = ti = None
-        if return_routing:
-            tw = torch.empty(M, topk, dtype=torch.float32, device=dev)
-            ti = torch.empty(M, topk, dtype=torch.int32, device=dev)
-        if M == 0:
-            return (out, tw, ti) if return_routing else out
-        lib = _lib.load()
-        nbytes = lib.fr_moe_decode_workspace_bytes(M, H, I, E, topk)
-        ws = _lib.call_workspace(nbytes, dev, "decode")
-        rc = lib.fr_moe_decode(_lib.ptr(hidden_states), _lib.ptr(gate), gate.stride(0), gate.stride(1), _lib.ptr(w1),
-                               _lib.ptr(s1), _lib.ptr(g1), _lib.ptr(w2), _lib.ptr(s2), _lib.ptr(g2),
-                               _lib.dtype_code(hidden_states.dtype), block, M, H, I, E, topk, 1 if renormalize else 0,
-                               _lib.ptr(out), _lib.ptr(tw), _lib.ptr(ti), _lib.ptr(ws), nbytes, _lib.stream_ptr(dev))
-    _lib.check(rc, "fr_moe_decode")
+    if _lib.elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _run(hidden_states, gate, w1, w2, dims, topk, renormalize, inplace, return_routing, block, s1, g1, s2, g2)
+    out = hidden_states if inplace else torch.empty_like(hidden_states)
+    tw = ti = None
+    if return_routing:
+        tw = torch.empty((M, topk), dtype=torch.float32, device=dev)
+        ti = torch.empty((M, topk), dtype=torch.int32, device=dev)
+    if M == 0:
+        return (out, tw, ti) if return_routing else out
+    lib = _lib.load()
+    nbytes = lib.fr_moe_decode_workspace_bytes(M, H, I, E, topk)
+    ws = _lib.call_workspace(nbytes, dev, "decode")
+    rc = lib.fr_moe_decode(hidden_states.data_ptr(), gate.data_ptr(), gate.stride(0), gate.stride(1), w1.data_ptr(),
+                           _lib.ptr(s1), _lib.ptr(g1), w2.data_ptr(), _lib.ptr(s2), _lib.ptr(g2),
+                           _lib.dtype_code(hidden_states.dtype), block, M, H, I, E, topk, 1 if renormalize else 0,
+                           out.data_ptr(), _lib.ptr(tw), _lib.ptr(ti), ws.data_ptr(), nbytes, _lib.stream_ptr(dev))
+    if rc:
+        _lib.check(rc, "fr_moe_decode")
     return (out, tw, ti) if return_routing else out
 
 

@@ -12,17 +12,21 @@ import torch
 
 from .. import _lib
 
+_SMALL = 32768      # elements of a matrix up to which one CTA quantises it, without a workspace
 _SCALE_DTYPE = {16: torch.float8_e4m3fn, 32: torch.float8_e8m0fnu}
+
+
+_BLOCK = {v: k for k, v in _SCALE_DTYPE.items()}
 
 
 def block_of(q: torch.Tensor, scale: torch.Tensor, what: str = "scale") -> int:
     """The block size of a quantised matrix, after checking that codes and scales belong together."""
     assert q.dtype == torch.uint8, "codes are packed in uint8"
-    assert scale.dtype in (torch.float8_e4m3fn, torch.float8_e8m0fnu), f"{what} must be float8_e4m3fn or float8_e8m0fnu"
-    block = 16 if scale.dtype == torch.float8_e4m3fn else 32
+    block = _BLOCK.get(scale.dtype)
+    assert block is not None, f"{what} must be float8_e4m3fn or float8_e8m0fnu"
     assert q.is_contiguous() and scale.is_contiguous(), f"codes and {what} must be contiguous"
-    assert scale.shape == (*q.shape[:-1], q.shape[-1] * 2 // block) and q.shape[-1] * 2 % block == 0, \
-        f"{what} does not match the codes"
+    a, b = q.shape, scale.shape
+    assert a[:-1] == b[:-1] and b[-1] * block == a[-1] * 2, f"{what} does not match the codes"
     return block
 
 
@@ -43,35 +47,40 @@ def quantize_fp4(x: torch.Tensor, block: int = 16, global_scale: torch.Tensor = 
     """
     _lib.require_cuda(x, global_scale)
     assert block in _SCALE_DTYPE, "block is 16 or 32"
-    assert x.dim() in (2, 3), "x is [rows, cols] or [mats, rows, cols]"
-    rows, cols = x.shape[-2:]
-    mats = x.shape[0] if x.dim() == 3 else 1
+    shape, dev = x.shape, x.device
+    dims = len(shape)
+    assert dims == 2 or dims == 3, "x is [rows, cols] or [mats, rows, cols]"
+    rows, cols = shape[-2], shape[-1]
+    mats = shape[0] if dims == 3 else 1
+    strides = x.stride()
     assert cols > 0 and cols % block == 0, f"the row length must be a multiple of {block}"
-    assert x.stride(-1) == 1, "the elements of a row must be adjacent"
+    assert strides[-1] == 1, "the elements of a row must be adjacent"
     assert block == 16 or global_scale is None, "block 32 has no global scale"
-    check_global(global_scale, mats, block)
-    dev = x.device
-    _lib.require_device(dev, global_scale)
-    lead = x.shape[:-1]
-    with _lib.on_device(dev):
-        q = torch.empty(*lead, cols // 2, dtype=torch.uint8, device=dev)
-        scale = torch.empty(*lead, cols // block, dtype=_SCALE_DTYPE[block], device=dev)
-        own = block == 16 and global_scale is None
-        if own:
-            global_scale = (torch.empty if rows else torch.ones)(mats, dtype=torch.float32, device=dev)
-        if mats == 0 or rows == 0:
-            return q, scale, global_scale
-        lib = _lib.load()
-        ws, nbytes = None, 0
-        if own:
-            nbytes = lib.fr_fp4_quantize_workspace_bytes(mats, rows, cols)
-            if nbytes:
-                ws = _lib.call_workspace(nbytes, dev, "fp4")
-        rc = lib.fr_fp4_quantize(_lib.ptr(x), _lib.dtype_code(x.dtype), mats, rows, cols,
-                                 x.stride(0) if x.dim() == 3 else 0, x.stride(-2) if rows > 1 else cols, block,
-                                 _lib.ptr(global_scale), 1 if own else 0, _lib.ptr(q), _lib.ptr(scale), _lib.ptr(ws),
-                                 nbytes, _lib.stream_ptr(dev))
-    _lib.check(rc, "fr_fp4_quantize")
+    if global_scale is not None:
+        check_global(global_scale, mats, block)
+        _lib.require_device(dev, global_scale)
+    if _lib.elsewhere(dev):
+        with torch.cuda.device(dev):
+            return quantize_fp4(x, block, global_scale)
+    lead = shape[:-1]
+    q = torch.empty((*lead, cols // 2), dtype=torch.uint8, device=dev)
+    scale = torch.empty((*lead, cols // block), dtype=_SCALE_DTYPE[block], device=dev)
+    own = block == 16 and global_scale is None
+    if own:
+        global_scale = (torch.empty if rows else torch.ones)(mats, dtype=torch.float32, device=dev)
+    if mats == 0 or rows == 0:
+        return q, scale, global_scale
+    lib = _lib.load()
+    ws, nbytes = None, 0
+    if own and rows * cols > _SMALL:
+        nbytes = lib.fr_fp4_quantize_workspace_bytes(mats, rows, cols)
+        ws = _lib.call_workspace(nbytes, dev, "fp4").data_ptr()
+    rc = lib.fr_fp4_quantize(x.data_ptr(), _lib.dtype_code(x.dtype), mats, rows, cols, strides[0] if dims == 3 else 0,
+                             strides[-2] if rows > 1 else cols, block,
+                             None if global_scale is None else global_scale.data_ptr(), 1 if own else 0, q.data_ptr(),
+                             scale.data_ptr(), ws, nbytes, _lib.stream_ptr(dev))
+    if rc:
+        _lib.check(rc, "fr_fp4_quantize")
     return q, scale, global_scale
 
 
@@ -79,21 +88,27 @@ def dequantize_fp4(q: torch.Tensor, scale: torch.Tensor, global_scale: torch.Ten
                    dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The numbers that codes and scales stand for, rounded once to ``dtype`` (fp16, bf16 or fp32)."""
     _lib.require_cuda(q, scale, global_scale)
-    assert q.dim() in (2, 3), "codes are [rows, cols/2] or [mats, rows, cols/2]"
+    shape, dev = q.shape, q.device
+    dims = len(shape)
+    assert dims == 2 or dims == 3, "codes are [rows, cols/2] or [mats, rows, cols/2]"
     block = block_of(q, scale)
-    rows, cols = q.shape[-2], q.shape[-1] * 2
-    mats = q.shape[0] if q.dim() == 3 else 1
-    check_global(global_scale, mats, block)
-    dev = q.device
-    _lib.require_device(dev, scale, global_scale)
+    rows, cols = shape[-2], shape[-1] * 2
+    mats = shape[0] if dims == 3 else 1
+    _lib.require_device(dev, scale)
+    if global_scale is not None:
+        check_global(global_scale, mats, block)
+        _lib.require_device(dev, global_scale)
     code = _lib.dtype_code(dtype)
-    with _lib.on_device(dev):
-        out = torch.empty(*q.shape[:-1], cols, dtype=dtype, device=dev)
-        if out.numel() == 0:
-            return out
-        rc = _lib.load().fr_fp4_dequantize(_lib.ptr(q), _lib.ptr(scale), _lib.ptr(global_scale), mats, rows, cols, block,
-                                           code, _lib.ptr(out), _lib.stream_ptr(dev))
-    _lib.check(rc, "fr_fp4_dequantize")
+    if _lib.elsewhere(dev):
+        with torch.cuda.device(dev):
+            return dequantize_fp4(q, scale, global_scale, dtype)
+    out = torch.empty((*shape[:-1], cols), dtype=dtype, device=dev)
+    if mats * rows * cols == 0:
+        return out
+    rc = _lib.load().fr_fp4_dequantize(q.data_ptr(), scale.data_ptr(), None if global_scale is None else global_scale.data_ptr(),
+                                       mats, rows, cols, block, code, out.data_ptr(), _lib.stream_ptr(dev))
+    if rc:
+        _lib.check(rc, "fr_fp4_dequantize")
     return out
 
 
@@ -110,27 +125,34 @@ def matmul_fp4(a_q: torch.Tensor, a_scale: torch.Tensor, b_q: torch.Tensor, b_sc
     m, n, k = a_q.shape[0], b_q.shape[0], a_q.shape[1] * 2
     assert b_q.shape[1] * 2 == k, "Incompatible dimensions"
     assert k > 0 and k % 32 == 0, "k must be a multiple of 32"
-    check_global(a_global, 1, block, "a_global")
-    check_global(b_global, 1, block, "b_global")
+    if a_global is not None:
+        check_global(a_global, 1, block, "a_global")
+    if b_global is not None:
+        check_global(b_global, 1, block, "b_global")
     dev = a_q.device
     _lib.require_device(dev, a_scale, b_q, b_scale, a_global, b_global, out)
     if out is not None:
         assert out.shape == (m, n) and out.dtype in (torch.float16, torch.bfloat16), "out is [m, n] in fp16 or bf16"
         assert out.stride(1) == 1 or n == 1, "the elements of a row of out must be adjacent"
         assert m <= 1 or out.stride(0) >= n, "rows of out must not overlap"
-    with _lib.on_device(dev):
-        if out is None:
-            assert dtype in (torch.float16, torch.bfloat16), f"unsupported dtype {dtype}"
-            out = torch.empty(m, n, dtype=dtype, device=dev)
-        if m == 0 or n == 0:
-            return out
-        lib = _lib.load()
+    if _lib.elsewhere(dev):
+        with torch.cuda.device(dev):
+            return matmul_fp4(a_q, a_scale, b_q, b_scale, a_global, b_global, dtype, out)
+    if out is None:
+        assert dtype in (torch.float16, torch.bfloat16), f"unsupported dtype {dtype}"
+        out = torch.empty((m, n), dtype=dtype, device=dev)
+    if m == 0 or n == 0:
+        return out
+    lib = _lib.load()
+    ws, nbytes = None, 0
+    if m > 128:                 # the library lays the scales out in a workspace
         nbytes = lib.fr_fp4_gemm_workspace_bytes(m, n, k, block)
-        ws = _lib.call_workspace(nbytes, dev, "fp4") if nbytes else None
-        rc = lib.fr_fp4_gemm(_lib.ptr(a_q), _lib.ptr(a_scale), _lib.ptr(a_global), _lib.ptr(b_q), _lib.ptr(b_scale),
-                             _lib.ptr(b_global), block, m, n, k, _lib.dtype_code(out.dtype), _lib.ptr(out),
-                             out.stride(0) if m > 1 else n, _lib.ptr(ws), nbytes, _lib.stream_ptr(dev))
-    _lib.check(rc, "fr_fp4_gemm")
+        ws = _lib.call_workspace(nbytes, dev, "fp4").data_ptr()
+    rc = lib.fr_fp4_gemm(a_q.data_ptr(), a_scale.data_ptr(), _lib.ptr(a_global), b_q.data_ptr(), b_scale.data_ptr(),
+                         _lib.ptr(b_global), block, m, n, k, _lib.dtype_code(out.dtype), out.data_ptr(),
+                         out.stride(0) if m > 1 else n, ws, nbytes, _lib.stream_ptr(dev))
+    if rc:
+        _lib.check(rc, "fr_fp4_gemm")
     return out
 
 
