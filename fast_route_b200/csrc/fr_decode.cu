@@ -2,12 +2,12 @@
 // weighted sum.  A batch this small reads every active expert's weights once and does almost no arithmetic per byte,
 // so the kernel is built around that stream:
 //
-//   logits -> grid barrier -> every CTA ranks all tokens (<= 16 KB of logits from L2) -> h = w1 x, act = silu(h_g) h_u
+//   logits, tagged with the call -> every CTA waits for all of them and ranks all tokens -> h = w1 x, act = silu(h_g) h_u
 //          -> grid barrier -> out = sum_e weight * (w2 act)
 //
 // * Work is split by weight ROWS, not by tiles: the (active experts * I) row pairs of w1 and the H rows of w2 are cut
-//   into equal contiguous ranges, so every CTA streams the same number of bytes whatever the sizes (16-row tiles left
-//   up to a quarter of the CTAs without a last tile).
+//   into equal contiguous ranges, so every CTA streams the same number of bytes whatever the sizes (16-row tiles would
+//   leave up to a quarter of the CTAs without a last tile).
 // * Each warp owns a FIFO in shared memory that it alone fills (cp.async, full 128-byte lines) and drains, so the
 //   stream needs no block barriers and runs on across row tiles, across experts and across the grid barrier: the first
 //   weights of w2 are in flight while the last activations are still being written.
@@ -39,7 +39,7 @@ constexpr int kDecScaleBytes = 512;                // and, for 4-bit weights, 32
 // the call used, so nothing has to be cleared in between).
 enum { DC_COUNT = 0, DC_BASE = 1, DC_FINISHED = 2, DC_BUDGET = 3, DC_EPOCH = 4, DC_GROUP = 64 /* one per row range */ };
 constexpr int kDecMaxGroups = 512;
-constexpr uint32_t kDecPolls = 1u << 22;           // about a second, unless DC_BUDGET holds another limit
+constexpr uint32_t kDecPolls = 1u << 22;           // a second or a few, unless DC_BUDGET holds another limit
 
 enum { WF_16BIT = 0, WF_NV4 = 1, WF_MX4 = 2 };
 
@@ -59,7 +59,7 @@ struct DecodeParams {
   uint16_t* out;
   float* tw;
   int32_t* ti;
-  unsigned int* control;         // DC_* below
+  unsigned int* control;         // DC_* above
   unsigned long long* logits;    // [M, E]: fp32 bits below, the call's tag above
   uint16_t* act;                 // [active expert][M][I]
 };
@@ -203,14 +203,22 @@ struct Fp4Expand {
 };
 
 // One token row's operand for the 64 bytes of weights a quad holds (16-bit weights: the lane's 8 elements, 4-bit: 32);
-// `p` points at the lane's first element.  Where `valid` is false the registers keep what they held: zeros, or earlier
-// elements of the same token.  Past the end of a row they meet weights of zero (and a NaN among them has made the
-// token's sum NaN already); for a token the expert does not get, the sums are not used.
-template <int WF>
-__device__ __forceinline__ void load_tokens(const uint16_t* p, bool valid, uint4 (&r)[WF == WF_16BIT ? 1 : 4]) {
-  if (!valid) return;
+// `p` points at the lane's first element.  For a token that the expert does not get (`use` false) the registers keep what
+// they held: its sums are not used.  Past the end of the row (`in` false) the weights are zero; where row lengths end
+// inside a step (RAGGED) the tokens' registers become zero as well, for an earlier infinity left in them would make a NaN
+// of that.  (A kernel of its own, since the test alone costs 1 to 6 % of the others; zeros first: written after the load
+// they would have to wait for it.)
+template <int WF, bool RAGGED>
+__device__ __forceinline__ void load_tokens(const uint16_t* p, bool use, bool in, uint4 (&r)[WF == WF_16BIT ? 1 : 4]) {
+  constexpr int NV = WF == WF_16BIT ? 1 : 4;
+  if (RAGGED && !in) {
 #pragma unroll
-  for (int v = 0; v < (WF == WF_16BIT ? 1 : 4); ++v) r[v] = *(reinterpret_cast<const uint4*>(p) + v);
+    for (int v = 0; v < NV; ++v) r[v] = make_uint4(0, 0, 0, 0);
+  }
+  if (use && in) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) r[v] = *(reinterpret_cast<const uint4*>(p) + v);
+  }
 }
 
 // acc += tokens * weights for one 16-byte chunk per lane of 16-bit weights
@@ -461,7 +469,8 @@ __device__ __forceinline__ void decode_finish(const DecodeParams& p, uint32_t ba
   }
 }
 
-template <bool BF16, int WF, bool HI>
+// RAGGED: rows of w1 or w2 end inside a step (of 128 or 256 bytes).
+template <bool BF16, int WF, bool HI, bool RAGGED>
 __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1)) moe_decode_kernel(const DecodeParams p) {
   extern __shared__ __align__(128) uint8_t dec_smem[];
   using C = DecodeCfg<WF, HI>;
@@ -652,8 +661,8 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
     if constexpr (WF != WF_16BIT) {
       if (left > 0 && warp < nb1) {
         const uint32_t mask = sm.mask[sm.list[a]];
-        load_tokens<WF>(x0, ((mask >> g) & 1u) && kb0 < rb1, lo[0]);
-        if constexpr (HI) load_tokens<WF>(x0 + x_hi, ((mask >> (g + 8)) & 1u) && kb0 < rb1, hi[0]);
+        load_tokens<WF, RAGGED>(x0, (mask >> g) & 1u, kb0 < rb1, lo[0]);
+        if constexpr (HI) load_tokens<WF, RAGGED>(x0 + x_hi, (mask >> (g + 8)) & 1u, kb0 < rb1, hi[0]);
       }
     }
     while (left > 0) {
@@ -673,8 +682,8 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
 #pragma unroll
           for (int st = 0; st < 2; ++st) {
             const bool in = kb + st * 64 < rb1;
-            load_tokens<WF>(xp + st * 4 * ELT, use_lo && in, lo[st]);
-            if constexpr (HI) load_tokens<WF>(xp + st * 4 * ELT + x_hi, use_hi && in, hi[st]);
+            load_tokens<WF, RAGGED>(xp + st * 4 * ELT, use_lo, in, lo[st]);
+            if constexpr (HI) load_tokens<WF, RAGGED>(xp + st * 4 * ELT + x_hi, use_hi, in, hi[st]);
           }
           const uint8_t *at, *no_scales;
           next_stage(at, no_scales);
@@ -700,8 +709,8 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
                 }
               }
             }
-            load_tokens<WF>(np, nl && in, lo[st ^ 1]);
-            if constexpr (HI) load_tokens<WF>(np + x_hi, nh && in, hi[st ^ 1]);
+            load_tokens<WF, RAGGED>(np, nl, in, lo[st ^ 1]);
+            if constexpr (HI) load_tokens<WF, RAGGED>(np + x_hi, nh, in, hi[st ^ 1]);
           };
           full_step4<BF16, WF, 4, 1>(acc, lo, hi, fetch, next_stage);
         }
@@ -813,8 +822,8 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
       const int kb = cur.b * (128 * LN2) + t4 * 16;
 #pragma unroll
       for (int st = 0; st < (WF == WF_16BIT ? 4 : 1); ++st) {
-        load_tokens<WF>(operand(cur) + st * 4 * ELT, routed(cur, g) && kb + st * 64 < rb2, lo[st]);
-        if constexpr (HI) load_tokens<WF>(operand(cur) + a_hi + st * 4 * ELT, routed(cur, g + 8) && kb + st * 64 < rb2, hi[st]);
+        load_tokens<WF, RAGGED>(operand(cur) + st * 4 * ELT, routed(cur, g), kb + st * 64 < rb2, lo[st]);
+        if constexpr (HI) load_tokens<WF, RAGGED>(operand(cur) + a_hi + st * 4 * ELT, routed(cur, g + 8), kb + st * 64 < rb2, hi[st]);
       }
     }
     while (cur.slot < n_active) {
@@ -830,15 +839,15 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
 #pragma unroll
           for (int st = 0; st < 4; ++st) {
             nlo[st][0] = lo[st][0];
-            load_tokens<WF>(np + st * 4 * ELT, use && nkb + st * 64 < rb2, nlo[st]);
+            load_tokens<WF, RAGGED>(np + st * 4 * ELT, use, more && nkb + st * 64 < rb2, nlo[st]);
           }
         } else {
           const uint16_t* ap = operand(cur);
           const bool use_lo = routed(cur, g), use_hi = routed(cur, g + 8);
 #pragma unroll
           for (int st = 0; st < 4; ++st) {
-            load_tokens<WF>(ap + st * 4 * ELT, use_lo && kb + st * 64 < rb2, lo[st]);
-            load_tokens<WF>(ap + st * 4 * ELT + a_hi, use_hi && kb + st * 64 < rb2, hi[st]);
+            load_tokens<WF, RAGGED>(ap + st * 4 * ELT, use_lo, kb + st * 64 < rb2, lo[st]);
+            load_tokens<WF, RAGGED>(ap + st * 4 * ELT + a_hi, use_hi, kb + st * 64 < rb2, hi[st]);
           }
         }
         const uint8_t *at, *no_scales;
@@ -861,8 +870,8 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
           constexpr int LAST = 2 * LN2 - 1;
           const bool in = st < LAST ? kb + (st + 1) * 64 < rb2 : more && nkb < rb2;
           const uint16_t* np = st < LAST ? ap + (st + 1) * 4 * ELT : nap;
-          load_tokens<WF>(np, (st < LAST ? use_lo : nuse_lo) && in, lo[(st & 1) ^ 1]);
-          if constexpr (HI) load_tokens<WF>(np + a_hi, (st < LAST ? use_hi : nuse_hi) && in, hi[(st & 1) ^ 1]);
+          load_tokens<WF, RAGGED>(np, st < LAST ? use_lo : nuse_lo, in, lo[(st & 1) ^ 1]);
+          if constexpr (HI) load_tokens<WF, RAGGED>(np + a_hi, st < LAST ? use_hi : nuse_hi, in, hi[(st & 1) ^ 1]);
         };
         full_step4<BF16, WF, NS2, LN2>(acc, lo, hi, fetch, next_stage);
       }
@@ -947,9 +956,9 @@ size_t moe_decode_workspace(int64_t M, int H, int I, int E, int topk) {
 }
 
 // HI: more than 8 tokens, the second half of the MMA's row side is used
-template <bool BF16, int WF, bool HI>
+template <bool BF16, int WF, bool HI, bool RAGGED>
 static int launch_decode_rows(const DecodeParams& p, cudaStream_t st) {
-  auto kern = moe_decode_kernel<BF16, WF, HI>;
+  auto kern = moe_decode_kernel<BF16, WF, HI, RAGGED>;
   constexpr int smem = sizeof(DecodeSmem<WF, HI>);
   // resident CTAs of the device, looked up once (0 = not yet)
   constexpr int kMaxDevices = 64;
@@ -988,7 +997,10 @@ static int launch_decode_rows(const DecodeParams& p, cudaStream_t st) {
 
 template <bool BF16, int WF>
 static int launch_decode(const DecodeParams& p, cudaStream_t st) {
-  return p.M > 8 ? launch_decode_rows<BF16, WF, true>(p, st) : launch_decode_rows<BF16, WF, false>(p, st);
+  const int per_line = WF == WF_16BIT ? 64 : 256;       // elements in 128 bytes
+  if (p.H % per_line || p.I % (2 * per_line))
+    return p.M > 8 ? launch_decode_rows<BF16, WF, true, true>(p, st) : launch_decode_rows<BF16, WF, false, true>(p, st);
+  return p.M > 8 ? launch_decode_rows<BF16, WF, true, false>(p, st) : launch_decode_rows<BF16, WF, false, false>(p, st);
 }
 
 int moe_decode_dispatch(const void* x, const void* gate, int64_t gsh, int64_t gse, const void* w1, const void* s1,

@@ -146,6 +146,23 @@ def test_nan_and_infinite_weights_stay_with_their_expert(dev):
     assert torch.equal(out[keep], clean[keep])
 
 
+@pytest.mark.parametrize("H,I", [(264, 200), (1000, 1000), (72, 520)])
+def test_infinities_past_the_end_of_a_row(dev, H, I):
+    """Row lengths that end inside a step, an infinity in the first elements: no NaN comes of a product with the filling."""
+    M, E, k = 3, 2, 2
+    g = torch.Generator().manual_seed(4)
+    for dt in (torch.bfloat16, torch.float16):
+        x = torch.rand(M, H, generator=g).to(dt)
+        w1, w2 = torch.rand(E, 2 * I, H, generator=g).to(dt) * 0.01, torch.rand(E, H, I, generator=g).to(dt) * 0.01 + 0.01
+        w1 += 0.01                                         # every weight positive: an infinity stays one
+        x[1, 5] = float("inf")
+        gate = torch.zeros(H, E, dtype=dt)                 # both experts, half each, for finite and infinite tokens alike
+        gate[:, 0] = 0
+        out = fr.fused_moe_decode(x.to(dev), gate.to(dev), w1.to(dev), w2.to(dev), k).cpu()
+        assert torch.isfinite(out[[0, 2]]).all()
+        assert torch.isinf(out[1]).all() and (out[1] > 0).all()
+
+
 def test_nan_scales_stay_with_their_expert(dev):
     M, H, I, E, k = 6, 256, 192, 8, 2
     x, gate, w1, w2 = (t.to(dev) for t in synth.moe_inputs(M, H, I, E, seed=3, dtype=torch.bfloat16, weight_std=0.05))
