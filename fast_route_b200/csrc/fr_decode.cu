@@ -469,6 +469,16 @@ __device__ __forceinline__ void decode_finish(const DecodeParams& p, uint32_t ba
   }
 }
 
+// The last act of a CTA whose wait ran out: it still arrives at its row range's counter, without which the range's next
+// calls would take a wrong CTA for the last one.
+__device__ __forceinline__ void decode_give_up(const DecodeParams& p, uint32_t base, uint32_t epoch) {
+  const int ks = static_cast<int>(blockIdx.x) / p.groups, group = static_cast<int>(blockIdx.x) - ks * p.groups;
+  if (threadIdx.x == 0 && p.ksplit > 1 && ks < p.ksplit &&
+      atomicAdd(p.control + DC_GROUP + group, 1u) == static_cast<unsigned int>(p.ksplit) - 1u)
+    p.control[DC_GROUP + group] = 0;
+  decode_finish(p, base, epoch);
+}
+
 // RAGGED: rows of w1 or w2 end inside a step (of 128 or 256 bytes).
 template <bool BF16, int WF, bool HI, bool RAGGED>
 __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1)) moe_decode_kernel(const DecodeParams p) {
@@ -495,7 +505,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
   if (!(p.E <= 64 ? decode_rank<2, NT>(p, sm, epoch + 1, sel, val)
                   : decode_rank<kDecMaxExperts / 32, NT>(p, sm, epoch + 1, sel, val))) {
     if (threadIdx.x == 0) atomicAdd(p.control + DC_COUNT, 1u);      // the others' barrier counts every CTA
-    decode_finish(p, base, epoch);
+    decode_give_up(p, base, epoch);
     return;
   }
   int n_active = 0;
@@ -775,7 +785,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
   __syncthreads();
   if (!sm.ok) {
     cp_async_wait<0>();
-    decode_finish(p, base, epoch);
+    decode_give_up(p, base, epoch);
     return;
   }
   // ---- GEMM2 + weighted sum over the experts ----

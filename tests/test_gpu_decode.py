@@ -307,6 +307,39 @@ def test_a_wait_that_runs_out_is_reported(dev):
     assert _lib.device_status()[0] == 0 and torch.equal(out, want)
 
 
+@pytest.mark.parametrize("polls", [1, 3, 10, 30, 100])
+def test_a_wait_that_runs_out_in_some_blocks_leaves_the_workspace_usable(dev, polls):
+    """With few polls some thread blocks give up and others do not.  Whatever the mixture, the same workspace serves the
+    next call: H = 256 has several blocks per row range of the second product, whose counters end at zero."""
+    from fast_route_b200 import _lib
+    M, H, I, E, k = 3, 256, 512, 8, 2
+    x, gate, w1, w2 = (t.to(dev) for t in synth.moe_inputs(M, H, I, E, seed=5, dtype=torch.bfloat16))
+    lib = _lib.load()
+    nbytes = lib.fr_moe_decode_workspace_bytes(M, H, I, E, k)
+    ws = torch.zeros(nbytes + 1024, dtype=torch.uint8, device=dev)
+    ws = ws[(-ws.data_ptr()) % 1024:][:nbytes]
+    out = torch.empty_like(x)
+
+    def call():
+        assert lib.fr_moe_decode(_lib.ptr(x), _lib.ptr(gate), gate.stride(0), gate.stride(1), _lib.ptr(w1), None, None,
+                                 _lib.ptr(w2), None, None, 1, 0, M, H, I, E, k, 1, _lib.ptr(out), None, None,
+                                 _lib.ptr(ws), nbytes, _lib.stream_ptr(dev)) == 0
+        torch.cuda.synchronize()
+        return _lib.device_status()[0]
+    assert call() == 0
+    want = out.clone()
+    words, counters = ws[:32].view(torch.int32), ws[256:256 + 4 * 128].view(torch.int32)
+    for _ in range(20):
+        words[3] = polls
+        assert call() in (0, 1)
+        assert int(words[0]) == int(words[1]) and int(words[2]) == 0
+        assert int(counters.abs().sum()) == 0
+        words[3] = 0
+        out.zero_()
+        assert call() == 0
+        assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("block,dt", [(16, torch.bfloat16), (32, torch.bfloat16)])
 @pytest.mark.parametrize("H,I", [(32, 32), (96, 160), (544, 224), (64, 2080)])
 def test_scales_that_start_anywhere(dev, H, I, block, dt):
