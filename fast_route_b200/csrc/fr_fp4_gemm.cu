@@ -142,6 +142,21 @@ __device__ __forceinline__ int fg_park(int swapped, int row, int col) {
   return swapped ? col * FG_LANES + row : row * (BN + 4) + col;
 }
 
+// The sums' factor ga * gb.  Where the product of the two leaves fp32's normal range (results need not: two matrices of
+// magnitude 1e-18), the second number holds half of its power of two: the first multiplication is then exact to fp32's
+// precision, and the second scales.
+struct FgAlpha {
+  float a, b;
+};
+__device__ __forceinline__ FgAlpha fg_alpha(const float* ga, const float* gb) {
+  const float x = ga ? __ldg(ga) : 1.0f, y = gb ? __ldg(gb) : 1.0f, xy = x * y;
+  if (fabsf(xy) >= 1.17549435e-38f && fabsf(xy) <= 3.40282347e38f) return {xy, 1.0f};
+  int ex, ey;
+  const float m = frexpf(x, &ex) * frexpf(y, &ey);
+  const int e = ex + ey, half = e / 2;
+  return {ldexpf(m, half), ldexpf(1.0f, e - half)};
+}
+
 template <int BN, int BLOCK, bool BF16>
 __global__ void __launch_bounds__((FgCfg<BN, BLOCK>::THREADS), 1)
 fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const FgParams p) {
@@ -335,7 +350,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     // ------------------------------ epilogue ----------------------------------
     const int q = warp & 3, half = (warp - C::EPI0) >> 2;       // lanes 32q .. 32q+31, columns of this half
     constexpr int HC = BN / 2 < 16 ? 16 : BN / 2;
-    const float alpha = (p.ga ? __ldg(p.ga) : 1.0f) * (p.gb ? __ldg(p.gb) : 1.0f);
+    const FgAlpha alpha = fg_alpha(p.ga, p.gb);
     uint32_t it = 0;
     for (int tile = first; tile < tiles; tile += stride, ++it) {
       const int64_t ra = static_cast<int64_t>(tile % p.tiles_a) * FG_LANES + q * 32 + lane;
@@ -374,7 +389,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         tc_wait_ld();
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          pk[c0 / 2 + i] = pack2<BF16>(__uint_as_float(v[2 * i]) * alpha, __uint_as_float(v[2 * i + 1]) * alpha);
+          pk[c0 / 2 + i] = pack2<BF16>(__uint_as_float(v[2 * i]) * alpha.a * alpha.b, __uint_as_float(v[2 * i + 1]) * alpha.a * alpha.b);
       }
       tc_fence_before();
       __syncwarp();
@@ -409,7 +424,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     __syncwarp();
     cluster.sync();
     const bool ok = *abort_flag == 0;
-    const float alpha = (p.ga ? __ldg(p.ga) : 1.0f) * (p.gb ? __ldg(p.gb) : 1.0f);
+    const FgAlpha alpha = fg_alpha(p.ga, p.gb);
     // slices of the tile's columns; BN / split is a multiple of 4
     const int cols = BN / p.split, c_lo = cols * rank;
     const int64_t ra0 = static_cast<int64_t>(first % p.tiles_a) * FG_LANES;
@@ -435,7 +450,8 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 #pragma unroll
       for (int s = 1; s < 8; ++s)
         if (s < p.split) v.x += f[s].x, v.y += f[s].y, v.z += f[s].z, v.w += f[s].w;
-      const uint32_t lo = pack2<BF16>(v.x * alpha, v.y * alpha), hi = pack2<BF16>(v.z * alpha, v.w * alpha);
+      const uint32_t lo = pack2<BF16>(v.x * alpha.a * alpha.b, v.y * alpha.a * alpha.b);
+      const uint32_t hi = pack2<BF16>(v.z * alpha.a * alpha.b, v.w * alpha.a * alpha.b);
       uint16_t* o = p.c + row * p.ldc + col;
       if (pairs4 && col + 4 <= width) {
         *reinterpret_cast<uint2*>(o) = make_uint2(lo, hi);

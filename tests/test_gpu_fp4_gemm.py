@@ -80,6 +80,25 @@ def test_every_scale_is_placed_right(dev, block, m):
     _check(fr.matmul_fp4(aq, asc, bq, bsc, ag, bg), ref, err)
 
 
+@pytest.mark.parametrize("ea,eb", [(-70, -72), (-30, -100), (-110, -60), (100, 60), (90, -110), (110, -149)])
+@pytest.mark.parametrize("m,k", [(3, 256), (3, 2048), (100, 2048), (260, 256), (260, 2048)])
+def test_global_scales_whose_product_leaves_fp32(dev, m, k, ea, eb):
+    """Results inside the output's range are as exact as ever, results past it are infinite, and rows of zeros stay zero."""
+    g = torch.Generator().manual_seed(m + k)
+    n = 150
+    (aq, asc, _), (bq, bsc, _) = _matrix(g, 16, m, k, wide=True), _matrix(g, 16, n, k, wide=True)
+    aq[1] = 0
+    a, b = (aq, asc, torch.tensor([1.3 * 2.0 ** ea])), (bq, bsc, torch.tensor([1.0 * 2.0 ** eb]))
+    ref, err = _ref(a, b, 16, k)
+    (aq, asc, ag), (bq, bsc, bg) = _dev(a, dev), _dev(b, dev)
+    c = fr.matmul_fp4(aq, asc, bq, bsc, ag, bg)
+    assert (c[1] == 0).all()
+    _check(c, ref, err)
+    top = float(torch.finfo(c.dtype).max)
+    sure = torch.from_numpy(np.abs(ref) - err > 1.01 * top)
+    assert torch.isinf(c.cpu()[sure]).all()
+
+
 @pytest.mark.parametrize("m", [7, 90, 260])
 def test_out_with_a_pitch_and_what_lies_around_it(dev, m):
     g = torch.Generator().manual_seed(5)
