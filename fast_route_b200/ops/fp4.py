@@ -42,7 +42,7 @@ def quantize_fp4(x: torch.Tensor, block: int = 16, global_scale: torch.Tensor = 
     -> ``(q[..., cols/2] uint8, scale[..., cols/block], global_scale)``.
 
     ``block=16``: ``global_scale`` (fp32, one per matrix) is computed from the largest magnitude, or taken from the
-    caller (a calibrated value: one pass over ``x`` less) and returned as given.  ``block=32`` has none (``None``).
+    caller (a calibrated positive value: one pass over ``x`` less) and returned as given.  ``block=32`` has none (``None``).
     A block holding an infinity or a NaN gets a NaN scale; such blocks do not enter the computed ``global_scale``.
     """
     _lib.require_cuda(x, global_scale)

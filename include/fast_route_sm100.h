@@ -296,7 +296,7 @@ int fr_w4a16_dequant(const int32_t* qweight, const void* scales, const int32_t* 
  * fr_fp4_quantize: x[mats][rows][cols] (FR_F16 / FR_BF16 / FR_F32; pitches ld_mat, ld_row in elements, elements of a
  *   row adjacent) -> q[mats][rows][cols / 2], scale[mats][rows][cols / block], dense.  block 16: with own_global != 0
  *   global_scale[mats] is computed (largest finite-block magnitude / 2688, 1 for a matrix of zeros, at least 2^-110)
- *   and written, else read; scale = e4m3(amax / (6 * global)), code = e2m1(x * (1 / (scale * global))).  block 32:
+ *   and written, else read (positive); scale = e4m3(amax / (6 * global)), code = e2m1(x * (1 / (scale * global))).  block 32:
  *   scale = 2^(floor(log2 amax) - 2), code = e2m1(x / scale) saturated at 6.  All roundings to nearest even, every
  *   operation a single fp32 rounding.  A block that holds an infinity or a NaN gets a NaN scale and zero codes.
  *   cols must be a multiple of block, mats <= 65535; workspace: fr_fp4_quantize_workspace_bytes (0 = none), needed with
