@@ -99,6 +99,20 @@ def test_global_scales_whose_product_leaves_fp32(dev, m, k, ea, eb):
     assert torch.isinf(c.cpu()[sure]).all()
 
 
+@pytest.mark.parametrize("m,n,k,pitch,lo", [(1111, 5001, 544, 5001, 0), (1111, 5000, 544, 5007, 3), (200, 263, 96, 264, 1),
+                                            (2500, 2049, 1024, 2050, 0)])
+def test_large_outputs_whose_rows_start_anywhere(dev, m, n, k, pitch, lo):
+    g = torch.Generator().manual_seed(n)
+    a, b = _matrix(g, 32, m, k), _matrix(g, 32, n, k)
+    (aq, asc, _), (bq, bsc, _) = _dev(a, dev), _dev(b, dev)
+    buf = torch.full((m + 2, pitch), 7.0, dtype=torch.bfloat16, device=dev)
+    out = buf[1:m + 1, lo:lo + n]
+    fr.matmul_fp4(aq, asc, bq, bsc, out=out)
+    _check(out, *_ref(a, b, 32, k))
+    out.fill_(7.0)
+    assert (buf == 7.0).all()
+
+
 @pytest.mark.parametrize("m", [7, 90, 260])
 def test_out_with_a_pitch_and_what_lies_around_it(dev, m):
     g = torch.Generator().manual_seed(5)
