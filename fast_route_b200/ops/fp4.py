@@ -72,13 +72,13 @@ def quantize_fp4(x: torch.Tensor, block: int = 16, global_scale: torch.Tensor = 
         return q, scale, global_scale
     lib = _lib.load()
     ws, nbytes = None, 0
-    if own and rows * cols > _SMALL:
+    if own and rows * cols > _SMALL:        # two launches: memory of this call's own, held until both are enqueued
         nbytes = lib.fr_fp4_quantize_workspace_bytes(mats, rows, cols)
-        ws = _lib.call_workspace(nbytes, dev, "fp4").data_ptr()
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     rc = lib.fr_fp4_quantize(x.data_ptr(), _lib.dtype_code(x.dtype), mats, rows, cols, strides[0] if dims == 3 else 0,
                              strides[-2] if rows > 1 else cols, block,
                              None if global_scale is None else global_scale.data_ptr(), 1 if own else 0, q.data_ptr(),
-                             scale.data_ptr(), ws, nbytes, _lib.stream_ptr(dev))
+                             scale.data_ptr(), _lib.ptr(ws), nbytes, _lib.stream_ptr(dev))
     if rc:
         _lib.check(rc, "fr_fp4_quantize")
     return q, scale, global_scale
@@ -145,12 +145,12 @@ def matmul_fp4(a_q: torch.Tensor, a_scale: torch.Tensor, b_q: torch.Tensor, b_sc
         return out
     lib = _lib.load()
     ws, nbytes = None, 0
-    if m > 128:                 # the library lays the scales out in a workspace
+    if m > 128:                 # the scales are laid out first: memory of this call's own, held until both are enqueued
         nbytes = lib.fr_fp4_gemm_workspace_bytes(m, n, k, block)
-        ws = _lib.call_workspace(nbytes, dev, "fp4").data_ptr()
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     rc = lib.fr_fp4_gemm(a_q.data_ptr(), a_scale.data_ptr(), _lib.ptr(a_global), b_q.data_ptr(), b_scale.data_ptr(),
                          _lib.ptr(b_global), block, m, n, k, _lib.dtype_code(out.dtype), out.data_ptr(),
-                         out.stride(0) if m > 1 else n, ws, nbytes, _lib.stream_ptr(dev))
+                         out.stride(0) if m > 1 else n, _lib.ptr(ws), nbytes, _lib.stream_ptr(dev))
     if rc:
         _lib.check(rc, "fr_fp4_gemm")
     return out
