@@ -1,0 +1,65 @@
+"""The 4-bit few-token layer at the ends of its scales' ranges, against the layer in 64 bits with the bound that follows from
+the kernel's rounding points (``oracle.fp4.layer_with_bound``)."""
+
+import numpy as np
+import pytest
+import torch
+
+import fast_route_b200 as fr
+from oracle import fp4 as o
+
+pytestmark = pytest.mark.gpu
+
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def _layer(M, H, I, E, block, scale1, scale2, size, seed, dt=torch.bfloat16):
+    """Random codes; block scales drawn from the byte ranges; rows of zeros in both matrices; tokens of magnitude ``size``.
+    The first element of a token meets zero codes only and decides the routing: expert weights from 1 to e^-30."""
+    g = torch.Generator().manual_seed(seed)
+
+    def matrix(rows, cols, scale):
+        q = torch.randint(0, 256, (E, rows, cols // 2), generator=g, dtype=torch.uint8)
+        s = torch.randint(scale[0], scale[1] + 1, (E, rows, cols // block), generator=g, dtype=torch.uint8)
+        return q, s
+    q1, s1 = matrix(2 * I, H, scale1)
+    q2, s2 = matrix(H, I, scale2)
+    q1[:, :, 0] &= 0xF0
+    q1[:, 3], q1[:, I + 8], q2[:, 5] = 0, 0, 0
+    x = (torch.randn(M, H, generator=g).to(torch.float64) * size).to(dt)
+    x[:, 0] = 1.0
+    gate = torch.zeros(H, E, dtype=dt)
+    gate[0] = torch.linspace(0, -30, E).to(dt)
+    return x, gate, q1, s1, q2, s2
+
+
+def _check(dev, x, gate, q1, s1, q2, s2, block, k, g1=None, g2=None):
+    sdt = E4M3 if block == 16 else E8M0
+    out, tw, ti = fr.fused_moe_decode_fp4(x.to(dev), gate.to(dev), q1.to(dev), s1.view(sdt).to(dev), q2.to(dev),
+                                          s2.view(sdt).to(dev), k, w1_global=None if g1 is None else g1.to(dev),
+                                          w2_global=None if g2 is None else g2.to(dev), return_routing=True)
+    w1, w2 = (o.values(q.numpy(), s.numpy(), None if g is None else g.double().numpy(), block)
+              for q, s, g in ((q1, s1, g1), (q2, s2, g2)))
+    ref, err = o.layer_with_bound(x.double().numpy(), w1, w2, ti.cpu().numpy(), tw.cpu().double().numpy(), torch.finfo(x.dtype).eps)
+    got = out.cpu().double().numpy()
+    top, tiny = float(torch.finfo(x.dtype).max), float(torch.finfo(x.dtype).smallest_normal)
+    sure = np.abs(ref) + err < top
+    assert sure.mean() > 0.9 and np.abs(ref[sure]).max() > 0
+    # below the type's normal numbers a rounding is off by at most half of `tiny * eps`: of the output, and of the
+    # activations, which the second matrix multiplies
+    slack = tiny * torch.finfo(x.dtype).eps * (1 + np.abs(w2).sum(-1).max(0))
+    assert (np.abs(got - ref) <= err + slack)[sure].all(), float((np.abs(got - ref) / (err + slack))[sure].max())
+    assert (got[:, 5] == 0).all()                    # a row of zeros gives zero, whatever the scales
+    return got
+
+
+@pytest.mark.parametrize("M", [2, 11])
+@pytest.mark.parametrize("H,I", [(256, 512), (288, 160)])
+@pytest.mark.parametrize("e1,size,e2", [(112, -118, 0), (116, -122, 112), (116, -126, 116), (-110, 104, 116), (-110, 100, -110),
+                                        (0, -6, 116), (122, -126, -100), (96, -102, 111)])
+def test_global_scales_at_the_ends_of_their_range(dev, M, H, I, e1, size, e2):
+    E, k = 4, 3
+    x, gate, q1, s1, q2, s2 = _layer(M, H, I, E, 16, (0x20, 0x48), (0x20, 0x38), 2.0 ** size, e1 + M)
+    g = torch.Generator().manual_seed(3)
+    g1, g2 = ((torch.rand(E, generator=g) * 0.9 + 1).double() * 2.0 ** e for e in (e1, e2))
+    _check(dev, x, gate, q1, s1, q2, s2, 16, k, g1.float(), g2.float())
