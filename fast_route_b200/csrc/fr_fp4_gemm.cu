@@ -154,8 +154,9 @@ __device__ __forceinline__ FgAlpha fg_alpha(const float* ga, const float* gb) {
   if (fabsf(xy) >= 1.17549435e-38f && fabsf(xy) <= 3.40282347e38f) return {xy, 1.0f};
   int ex, ey;
   const float m = frexpf(x, &ex) * frexpf(y, &ey);
+  // (at most 2^127 in the second: sums are zero or at least 2^-20, so nothing else than zero is finite from 2^255 on)
   const int e = ex + ey, half = e / 2;
-  return {ldexpf(m, half), ldexpf(1.0f, e - half)};
+  return {ldexpf(m, half), ldexpf(1.0f, min(e - half, 127))};
 }
 
 // ANY: rows of c may start anywhere (not swapped, one CTA per tile); a kernel of its own, for as a branch it costs the
