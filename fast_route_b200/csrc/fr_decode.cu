@@ -202,19 +202,13 @@ struct Fp4Expand {
   }
 };
 
-// What a sum of 4-bit weights is multiplied with: `weight` (a routing weight, at most 1) * global * kUnit, as a * b.  b is 1
-// unless that product leaves fp32's range, which results need not do: a matrix of magnitude 1e38 has a global scale of
-// 2^116, and kUnit of it is too much, while its rows of zeros stay zero and small tokens give ordinary results.  Then b is
-// kUnit, and sums that overflow with it alone belong to results that overflow too.
-struct Fp4Factor {
-  float a, b;
-};
+// Sums of 4-bit weights are multiplied with global * kUnit.  That leaves fp32's range for global scales from 2^112 on (bf16,
+// blocks of 16: the only case with both), while results need not: a matrix of magnitude 1e37 has such a scale, but rows of
+// zeros stay zero and small tokens give ordinary results.  Then the two are applied one after the other.  (Decided for the
+// whole warp by the expert's scale: a factor of two parts for everybody costs 2 %.)
 template <bool BF16, int WF>
-__device__ __forceinline__ Fp4Factor fp4_factor(float weight, float global) {
-  constexpr float U = Fp4Expand<BF16, WF>::kUnit;
-  const float f = weight * U * global;
-  if (fabsf(f) <= 3.40282347e38f || f != f) return {f, 1.0f};
-  return {weight * global, U};
+__device__ __forceinline__ bool fp4_wide_global(float global) {
+  return BF16 && WF == WF_NV4 && fabsf(global) > 3.40282347e38f / Fp4Expand<BF16, WF>::kUnit;
 }
 
 // One token row's operand for the 64 bytes of weights a quad holds (16-bit weights: the lane's 8 elements, 4-bit: 32);
@@ -767,9 +761,9 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
           }
           if constexpr (WF != WF_16BIT) {
             const float gl = p.g1 ? __ldg(p.g1 + e) : 1.0f;
-            const Fp4Factor f = fp4_factor<BF16, WF>(1.0f, gl);
-            hg = hg * f.a * f.b;
-            hu = hu * f.a * f.b;
+            constexpr float U = Fp4Expand<BF16, WF>::kUnit;
+            if (fp4_wide_global<BF16, WF>(gl)) hg = hg * gl * U, hu = hu * gl * U;
+            else hg *= gl * U, hu *= gl * U;
           }
           const uint32_t v = pack2<BF16>(silu_f(hg) * hu, 0.0f);
           p.act[(static_cast<int64_t>(a) * p.M + t) * p.I + j0 + j] = static_cast<uint16_t>(v);
@@ -818,18 +812,21 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
     auto fold = [&](int from) {
       const int e = sm.list[from];
       const uint32_t mask = sm.mask[e];
-      float w_lo = sm.weight[e][g], w_hi = HI ? sm.weight[e][(g + 8) % C::TOKENS] : 0.0f;
+      float f = 1.0f, last = 1.0f;
+      bool wide = false;
       if constexpr (WF != WF_16BIT) {
+        last = Fp4Expand<BF16, WF>::kUnit;
         const float gl = p.g2 ? __ldg(p.g2 + e) : 1.0f;
-        const Fp4Factor lo = fp4_factor<BF16, WF>(w_lo, gl), hi = fp4_factor<BF16, WF>(w_hi, gl);
-        w_lo = lo.a;
-        w_hi = hi.a;
-        if (lo.b != 1.0f || hi.b != 1.0f) {
+        wide = fp4_wide_global<BF16, WF>(gl);
+        f = wide ? gl : gl * last;
+      }
+      float w_lo = sm.weight[e][g] * f, w_hi = HI ? sm.weight[e][(g + 8) % C::TOKENS] * f : 0.0f;
+      if (wide) {
 #pragma unroll
-          for (int s = 0; s < NS2; ++s)
+        for (int s = 0; s < NS2; ++s)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[s][i] *= i < 2 ? lo.b : hi.b;
-        }
+          for (int i = 0; i < 4; ++i) acc[s][i] *= i < 2 ? w_lo : w_hi;
+        w_lo = w_hi = last;
       }
 #pragma unroll
       for (int s = 0; s < NS2; ++s) {
