@@ -146,14 +146,14 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
 template <bool BF16, int WF>
 struct Fp4Expand {
   // what is left to multiply the sums with: the factors below keep every intermediate inside the 16-bit format
-  static constexpr float kUnit = WF == WF_MX4 ? 4294967296.0f /* 2^32 */ : (BF16 ? 65536.0f : 1.0f);
+  static constexpr uint32_t kMx4Top = 133;
+  static constexpr float kUnit = WF == WF_MX4 ? 32.0f : (BF16 ? 65536.0f : 1.0f);
   // the factors of a lane's 32 codes: two blocks of 16 (m[0], m[1]) or one of 32
   static __device__ __forceinline__ void mult(uint32_t scales, uint32_t (&m)[2]) {
     if constexpr (WF == WF_MX4) {
-      // bf16 only: 2^(byte - 127) * 2^94.  Scales above 2^33 overflow to infinity; far below 2^-60 the products with
-      // small activations leave the fp32 range.
-      const uint32_t e = scales + 94;
-      const uint32_t b = scales == 0xFFu ? 0x7FC0u : (e < 255u ? e << 7 : 0x7F80u);
+      // bf16 only: 2^(byte - 127) * 2^121.  That reaches from the smallest scale, whose 0.5 is a subnormal bf16 number, to
+      // 2^6 (byte 133); what comes of larger scales and of NaN is not used: fp4_dot sums their tiles.
+      const uint32_t b = (scales + 121u) << 7;
       m[0] = m[1] = b | (b << 16);
     } else {
       uint32_t h;   // both scales in fp16, exact, NaN included
@@ -201,6 +201,33 @@ struct Fp4Expand {
     for (int j = 0; j < 4; ++j) o[j] = mul(o[j], m);
   }
 };
+
+// sum of n (a multiple of 32) products of E8M0-scaled codes and 16-bit numbers in fp32: for the tiles with scales beyond 2^6
+// (weights of 512 and more), which no trained layer is known to have, so it is short rather than fast (all of a layer in
+// such scales: 1650 us instead of 91 for 1 token of 8 experts, 1880 instead of 158 for 16 tokens of 64; a second factor in
+// the expansion costs everybody 11 to 14 %, behind a branch 4 to 8).
+static __device__ __noinline__ float fp4_dot(const uint8_t* codes, const uint8_t* scales, const uint16_t* x, int n) {
+  float sum = 0.0f;
+  for (int k = 0; k < n; k += 32) {
+    const float unit = e8m0_f32(__ldg(scales + k / 32));
+    const uint4 w = __ldg(reinterpret_cast<const uint4*>(codes + k / 2));
+    const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 v = *reinterpret_cast<const uint4*>(x + k + 8 * i);
+      const uint32_t pair[4] = {v.x, v.y, v.z, v.w};
+      uint32_t h[4];
+      cvt8_f16(word[i], h);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 c = unpack2<false>(h[j]), t = unpack2<true>(pair[j]);
+        sum = fmaf(__fmul_rn(c.x, unit), t.x, sum);
+        sum = fmaf(__fmul_rn(c.y, unit), t.y, sum);
+      }
+    }
+  }
+  return sum;
+}
 
 // Sums of 4-bit weights are multiplied with global * kUnit.  That leaves fp32's range for global scales from 2^112 on (bf16,
 // blocks of 16: the only case with both), while results need not: a matrix of magnitude 1e37 has such a scale, but rows of
@@ -266,10 +293,10 @@ __device__ __forceinline__ void chunk_mma4(float (&acc)[NS][4], const uint4 (&w)
 
 // One stage (LN lines of 128 bytes of every row of NS sub-tiles) of 4-bit weights, in half lines with two operand buffers
 // in turn: `fetch(st)` requests the operand of the half line after st into the buffer that st does not use, `stage` waits
-// for the weights and says where the lane's first chunk and scales are.
+// for the weights and says where the lane's first chunk and scales are.  `top_scale`: the largest E8M0 scale so far.
 template <bool BF16, int WF, int NS, int LN, class Fetch, class Stage>
 __device__ __forceinline__ void full_step4(float (&acc)[NS][4], const uint4 (&lo)[2][4], const uint4 (&hi)[2][4],
-                                           Fetch fetch, Stage stage) {
+                                           Fetch fetch, Stage stage, uint32_t& top_scale) {
   constexpr int SCB = WF == WF_NV4 ? 16 : 8;
   const uint8_t* at = nullptr;
   const uint8_t* sc_at = nullptr;
@@ -285,6 +312,7 @@ __device__ __forceinline__ void full_step4(float (&acc)[NS][4], const uint4 (&lo
       w[s] = *reinterpret_cast<const uint4*>(half + s * 1024);
       const uint8_t* q = sc_at + (s + (st >> 1) * NS) * 8 * SCB + (st & 1) * (SCB / 2);
       sc[s] = WF == WF_NV4 ? *reinterpret_cast<const uint16_t*>(q) : *q;
+      if constexpr (WF == WF_MX4) top_scale = max(top_scale, sc[s]);
     }
     chunk_mma4<BF16, WF, NS>(acc, w, sc, lo[st & 1], hi[st & 1]);
   }
@@ -651,6 +679,13 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
     cp_async_commit();
     ld_at = ld_at == (kDecStages - 1) * STAGE ? 0 : ld_at + STAGE;
   };
+  // E8M0: the largest scale of a tile is that of all slots, also of those past its rows, which hold nothing yet
+  uint32_t top_scale = 0;
+  if constexpr (WF == WF_MX4) {
+    for (int s = 0; s < kDecStages; ++s)
+      *reinterpret_cast<uint2*>(&sm.ring[warp][s][kDecCodeBytes + lane * SCB]) = make_uint2(0, 0);
+    __syncwarp();
+  }
   // the reading end: lane (g, t4) takes chunk t4 + 4 * st of row g of a sub-tile
   const uint8_t* fifo = &sm.ring[warp][0][0] + g * 128 + ((t4 ^ ((g & 1) << 2)) << 4);
   auto next_stage = [&](const uint8_t*& at, const uint8_t*& sc_at) {
@@ -659,6 +694,17 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
     at = fifo + at_off;
     sc_at = &sm.ring[warp][0][0] + at_off + kDecCodeBytes + g * SCB + t4 * (SCB / 8);
     at_off = at_off == (kDecStages - 1) * STAGE ? 0 : at_off + STAGE;
+  };
+  // the barrier behind a tile; true: the tile has scales that need fp4_dot
+  auto tile_done = [&]() {
+    if constexpr (WF == WF_MX4) {
+      const bool any = __syncthreads_or(top_scale > Fp4Expand<BF16, WF>::kMx4Top) != 0;
+      top_scale = 0;
+      return any;
+    } else {
+      __syncthreads();
+      return false;
+    }
   };
   auto chunk = [&](const uint8_t* at, int st) {   // st: 0 or 1; the other half of a row is at ^ 64
     return *reinterpret_cast<const uint4*>(st ? reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(at) ^ 64) : at);
@@ -731,7 +777,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
             load_tokens<WF, RAGGED>(np, nl, in, lo[st ^ 1]);
             if constexpr (HI) load_tokens<WF, RAGGED>(np + x_hi, nh, in, hi[st ^ 1]);
           };
-          full_step4<BF16, WF, 4, 1>(acc, lo, hi, fetch, next_stage);
+          full_step4<BF16, WF, 4, 1>(acc, lo, hi, fetch, next_stage, top_scale);
         }
         __syncwarp();
         issue();
@@ -748,7 +794,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
           o[PS + 8] = acc[s][3];
         }
       }
-      __syncthreads();
+      const bool dots = tile_done();
       {
         const int j = threadIdx.x & 15, t = threadIdx.x >> 4;   // t >= M: the mask has no such bit
         if (j < cnt && ((mask >> t) & 1u)) {
@@ -764,6 +810,12 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
             constexpr float U = Fp4Expand<BF16, WF>::kUnit;
             if (fp4_wide_global<BF16, WF>(gl)) hg = hg * gl * U, hu = hu * gl * U;
             else hg *= gl * U, hu *= gl * U;
+          }
+          if (dots) {
+            const int64_t row = static_cast<int64_t>(e) * 2 * p.I + j0 + j;
+            const uint16_t* xr = p.x + static_cast<int64_t>(t) * p.H;
+            hg = fp4_dot(p.w1 + row * rb1, p.s1 + row * sb1, xr, p.H);
+            hu = fp4_dot(p.w1 + (row + p.I) * rb1, p.s1 + (row + p.I) * sb1, xr, p.H);
           }
           const uint32_t v = pack2<BF16>(silu_f(hg) * hu, 0.0f);
           p.act[(static_cast<int64_t>(a) * p.M + t) * p.I + j0 + j] = static_cast<uint16_t>(v);
@@ -906,7 +958,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
           load_tokens<WF, RAGGED>(np, st < LAST ? use_lo : nuse_lo, in, lo[(st & 1) ^ 1]);
           if constexpr (HI) load_tokens<WF, RAGGED>(np + a_hi, st < LAST ? use_hi : nuse_hi, in, hi[(st & 1) ^ 1]);
         };
-        full_step4<BF16, WF, NS2, LN2>(acc, lo, hi, fetch, next_stage);
+        full_step4<BF16, WF, NS2, LN2>(acc, lo, hi, fetch, next_stage, top_scale);
       }
       __syncwarp();
       issue();
@@ -923,13 +975,24 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
         o[PS + 8] = tot[s][3];
       }
     }
-    __syncthreads();
+    const bool dots = tile_done();
     for (int i = threadIdx.x; i < 8 * NS2 * p.M; i += kDecThreads) {
       const int r = i % (8 * NS2), t = i / (8 * NS2);
       if (r0 + r < row1) {
         float v = 0.0f;
 #pragma unroll
         for (int w = 0; w < kDecWarps; ++w) v += sm.part[0][w][r * PS + t];
+        if (dots) {                // this CTA's double steps of every expert that has the token
+          v = 0.0f;
+          constexpr int KS = 128 * LN2 * 2;
+          for (int q = ks * kDecWarps; q < n_active * nb2; q = (q + 1) % kDecWarps ? q + 1 : q + 1 + n2nd - kDecWarps) {
+            const int slot = q / nb2, k = (q - slot * nb2) * KS, e = sm.list[slot];
+            if (!((sm.mask[e] >> t) & 1u)) continue;
+            const int64_t row = static_cast<int64_t>(e) * p.H + r0 + r;
+            v = fmaf(sm.weight[e][t], fp4_dot(p.w2 + row * rb2 + k / 2, p.s2 + row * sb2 + k / 32,
+                                              p.act + (static_cast<int64_t>(slot) * p.M + t) * p.I + k, min(KS, p.I - k)), v);
+          }
+        }
         const int64_t at = static_cast<int64_t>(t) * p.H + r0 + r;
         if (p.ksplit == 1) p.out[at] = static_cast<uint16_t>(pack2<BF16>(v, 0.0f));
         else __stcg(p.partial + static_cast<int64_t>(ks) * p.M * p.H + at, v);

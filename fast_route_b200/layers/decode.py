@@ -70,8 +70,9 @@ def fused_moe_decode_fp4(hidden_states: torch.Tensor, gate: torch.Tensor, w1_q: 
                          return_routing: bool = False):
     """The same with 4-bit experts: ``w1_q[E,2I,H/2]``, ``w2_q[E,H,I/2]`` and their block scales as ``quantize_fp4`` returns
     them for ``w1[E,2I,H]`` / ``w2[E,H,I]``; ``w1_global`` / ``w2_global`` hold one fp32 scale per expert (block 16;
-    ``None`` = 1).  The expanded weights are exact 16-bit numbers.  Block 32 (E8M0) needs bf16 activations and block
-    scales between 2^-60 and 2^33.  ``H`` and ``I`` are multiples of 32."""
+    ``None`` = 1).  The expanded weights are exact 16-bit numbers.  Block 32 (E8M0) needs bf16 activations; block scales
+    above 2^6 (weights of 512 and more) are right but slow, and weights of 2^128 and more are infinite, as
+    ``dequantize_fp4`` gives them.  ``H`` and ``I`` are multiples of 32."""
     assert hidden_states.dim() == 2 and gate.dim() == 2 and w1_q.dim() == 3 and w2_q.dim() == 3
     assert hidden_states.is_contiguous(), "Hidden_states must be contiguous"
     assert hidden_states.dtype in [torch.float16, torch.bfloat16] and gate.dtype == hidden_states.dtype

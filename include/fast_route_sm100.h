@@ -327,7 +327,7 @@ int fr_fp4_gemm(const void* a_q, const void* a_scale, const float* a_global, con
  *   block 16 / 32: w1 / w2 packed codes as fr_fp4_quantize writes them with mats = E (block scales w1_scale
  *   [E,2I,H/block], w2_scale [E,H,I/block]; block 16: w1_global / w2_global fp32[E], NULL = 1).  The activations stay in
  *   `dtype` and the expanded weights are exact, so nothing but the weights' own quantisation is lost.  Block 32 needs
- *   FR_BF16 and block scales between 2^-60 and 2^33.
+ *   FR_BF16; 16-row tiles with a block scale above 2^6 are summed by slower code, and weights of 2^128 and more are infinite.
  * x[M,H] dense; gate as in fr_route_fused; out[M,H] may alias x.  topk_weights_out / topk_ids_out: both or neither.
  * E <= 256; H and I multiples of 8 (block 0) or 32.  The workspace (256-byte aligned) starts with the control words of
  * the grid barrier: zero it once before its first use (see fr_align); one workspace serves one stream at a time. */
