@@ -63,6 +63,7 @@ SIGNATURES = {
     "fr_fp4_gemm_workspace_bytes": (_Z, [_L, _L, _L, _I]),
     "fr_fp4_gemm": (_I, [_P, _P, _P, _P, _P, _P, _I, _L, _L, _L, _I, _P, _L, _P, _Z, _P]),
     "fr_moe_decode_workspace_bytes": (_Z, [_L, _I, _I, _I, _I]),
+    "fr_moe_decode_state_bytes": (_Z, []),
     "fr_moe_decode": (_I, [_P, _P, _L, _L, _P, _P, _P, _P, _P, _P, _I, _I, _L, _I, _I, _I, _I, _I, _P, _P, _P, _P, _Z, _P]),
 }
 
@@ -168,11 +169,13 @@ def workspace(nbytes: int, device, tag: str = "layer") -> torch.Tensor:
     return buf[off:off + max(nbytes, 1)]
 
 
-def call_workspace(nbytes: int, device, tag: str) -> torch.Tensor:
-    """``workspace`` for calls that may be captured: inside a stream capture every call gets zeroed memory of its own
-    from the graph's pool, so that two graphs replayed side by side share none.  ``device`` is the current one."""
+def call_workspace(nbytes: int, device, tag: str, state_bytes) -> torch.Tensor:
+    """``workspace`` for calls that may be captured: inside a stream capture every call gets memory of its own from the
+    graph's pool, so that two graphs replayed side by side share none.  Every replay clears the first ``state_bytes()``
+    bytes, which is all that such a workspace has to be cleared of.  ``device`` is the current one."""
     if not torch.cuda.is_current_stream_capturing():
         return workspace(nbytes, device, tag)
-    buf = torch.zeros(int(nbytes) + 1024, dtype=torch.uint8, device=device)
+    buf = torch.empty(int(nbytes) + 1024, dtype=torch.uint8, device=device)
     off = (-buf.data_ptr()) % 1024
+    buf[off:off + state_bytes()].zero_()
     return buf[off:off + max(nbytes, 1)]

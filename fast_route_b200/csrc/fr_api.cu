@@ -1498,6 +1498,8 @@ size_t fr_moe_decode_workspace_bytes(int64_t M, int H, int I, int E, int topk) {
   return fr::moe_decode_workspace(M, H, I, E, topk);
 }
 
+size_t fr_moe_decode_state_bytes(void) { return fr::moe_decode_state(); }
+
 int fr_moe_decode(const void* x, const void* gate, int64_t gate_stride_h, int64_t gate_stride_e, const void* w1,
                   const void* w1_scale, const float* w1_global, const void* w2, const void* w2_scale,
                   const float* w2_global, int dtype, int block, int64_t M, int H, int I, int E, int topk,

@@ -1046,6 +1046,8 @@ static DecodeWs decode_ws(int64_t M, int H, int I, int E, int topk) {
   return w;
 }
 
+size_t moe_decode_state() { return decode_ws(1, 1, 1, 1, 1).partial; }    // control words and tagged logits: the same for all sizes
+
 size_t moe_decode_workspace(int64_t M, int H, int I, int E, int topk) {
   if (M <= 0 || M > kDecTokens || H <= 0 || I <= 0 || E <= 0 || topk <= 0 || topk > E) return 0;
   return decode_ws(M, H, I, E, topk).total;

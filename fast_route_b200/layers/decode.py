@@ -34,7 +34,7 @@ def _run(hidden_states, gate, w1, w2, dims, topk, renormalize, inplace, return_r
         return (out, tw, ti) if return_routing else out
     lib = _lib.load()
     nbytes = lib.fr_moe_decode_workspace_bytes(M, H, I, E, topk)
-    ws = _lib.call_workspace(nbytes, dev, "decode")
+    ws = _lib.call_workspace(nbytes, dev, "decode", lib.fr_moe_decode_state_bytes)
     rc = lib.fr_moe_decode(hidden_states.data_ptr(), gate.data_ptr(), gate.stride(0), gate.stride(1), w1.data_ptr(),
                            _lib.ptr(s1), _lib.ptr(g1), w2.data_ptr(), _lib.ptr(s2), _lib.ptr(g2),
                            _lib.dtype_code(hidden_states.dtype), block, M, H, I, E, topk, 1 if renormalize else 0,

@@ -330,9 +330,11 @@ int fr_fp4_gemm(const void* a_q, const void* a_scale, const float* a_global, con
  *   FR_BF16; 16-row tiles with a block scale above 2^6 are summed by slower code, and weights of 2^128 and more are infinite.
  * x[M,H] dense; gate as in fr_route_fused; out[M,H] may alias x.  topk_weights_out / topk_ids_out: both or neither.
  * E <= 256; H and I multiples of 8 (block 0) or 32.  The workspace (256-byte aligned) starts with the control words of
- * the grid barrier: zero it once before its first use (see fr_align); one workspace serves one stream at a time. */
+ * the grid barrier and the tagged logits: zero its first fr_moe_decode_state_bytes once before its first use (see fr_align);
+ * the rest needs no initial state.  One workspace serves one stream at a time. */
 #define FR_DECODE_MAX_TOKENS 16
 size_t fr_moe_decode_workspace_bytes(int64_t M, int H, int I, int E, int topk);
+size_t fr_moe_decode_state_bytes(void);
 int fr_moe_decode(const void* x, const void* gate, int64_t gate_stride_h, int64_t gate_stride_e, const void* w1,
                   const void* w1_scale, const float* w1_global, const void* w2, const void* w2_scale,
                   const float* w2_global, int dtype, int block, int64_t M, int H, int I, int E, int topk,

@@ -93,3 +93,18 @@ def test_two_calls_at_once_have_scratch_of_their_own(library, first, second):
     (a0, a1, a_held), (b0, b1, b_held) = library.scratch.values()
     assert a1 <= b0 or b1 <= a0, "both calls use the same memory"
     assert a_held and b_held, "the memory was given back while its call was running"
+
+
+def test_a_captured_call_clears_its_state_only(lib, monkeypatch):
+    """Inside a capture every replay repeats the clearing: the few-token layer's control words and logits, not the rest."""
+    state = lib.fr_moe_decode_state_bytes()
+    nbytes = lib.fr_moe_decode_workspace_bytes(16, 2048, 1408, 64, 6)
+    assert 0 < state < 40000 < (1 << 20) < nbytes
+    for sizes in ((1, 64, 64, 4, 2), (16, 4096, 14336, 256, 8)):        # the state has the same place at every size
+        assert lib.fr_moe_decode_workspace_bytes(*sizes) > state
+    empty = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: empty(*a, **kw).fill_(7))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    ws = _lib.call_workspace(nbytes, torch.device("cpu"), "decode", lib.fr_moe_decode_state_bytes)
+    assert ws.numel() == nbytes and ws.data_ptr() % 256 == 0
+    assert not ws[:state].any() and (ws[state:] == 7).all()
