@@ -159,6 +159,25 @@ __device__ __forceinline__ FgAlpha fg_alpha(const float* ga, const float* gb) {
   return {ldexpf(m, half), ldexpf(1.0f, min(e - half, 127))};
 }
 
+// After a wait that ran out: copies and MMAs that are still in flight end before their memory is given back, each stage's
+// last fill and what every issuing thread has issued.  Bounded again, by some milliseconds for what takes microseconds.
+// (A stage whose scale loaders gave up never becomes full.)  Not inlined: its registers are none of the kernel's.
+static __device__ __noinline__ void fg_drain(uint64_t* full, uint64_t* drained, uint32_t produced, int stages, int issuers) {
+  auto wait = [](uint64_t* bar, uint32_t parity) {
+    for (uint32_t it = 0; it < (1u << 14); ++it)
+      if (mbar_try_wait(bar, parity)) return;
+  };
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    const int stage = static_cast<int>(produced & 0xFFu);
+    for (int s = 0; s < stages; ++s) wait(full + s, (produced >> 8) ^ (s < stage ? 0u : 1u));
+  } else if ((threadIdx.x & 31) == 0 && warp >= 1 && warp <= issuers) {
+    tc_commit(drained + warp - 1);
+    wait(drained + warp - 1, 0);
+  }
+  __syncthreads();
+}
+
 // ANY: rows of c may start anywhere (not swapped, one CTA per tile); a kernel of its own, for as a branch it costs the
 // other case 3 % (registers).
 template <int BN, int BLOCK, bool BF16, bool ANY>
@@ -173,8 +192,10 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   uint64_t* sfull = empty + S;            // scales of the stage are in tensor memory (two issuers)
   uint64_t* tfull = sfull + S;
   uint64_t* tempty = tfull + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 1);
+  uint64_t* drained = tempty + 1;         // of the issuing threads, used after a wait that ran out
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 3);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile uint32_t* produced = tmem_slot + 2;   // where the producer stopped: stage, and its phase in bit 8
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -185,6 +206,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     }
     mbar_init(tfull, C::ISSUERS);
     mbar_init(tempty, 8);
+    for (int w = 0; w < 3; ++w) mbar_init(&drained[w], 1);
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmA);
@@ -235,6 +257,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           ps.advance_rt(S);
         }
       }
+      *produced = ps.stage | (ps.phase << 8);
     }
   } else if (warp <= C::ISSUERS) {
     // ------------------------------ MMA issuers -------------------------------
@@ -488,6 +511,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   }
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag) fg_drain(full, drained, *produced, S, C::ISSUERS + (C::ISSUERS > 1 ? 1 : 0));
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, C::TMEM_COLS);
