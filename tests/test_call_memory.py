@@ -108,3 +108,16 @@ def test_a_captured_call_clears_its_state_only(lib, monkeypatch):
     ws = _lib.call_workspace(nbytes, torch.device("cpu"), "decode", lib.fr_moe_decode_state_bytes)
     assert ws.numel() == nbytes and ws.data_ptr() % 256 == 0
     assert not ws[:state].any() and (ws[state:] == 7).all()
+
+
+def test_sizes_that_need_scratch_are_the_librarys(lib):
+    """``quantize_fp4`` and ``matmul_fp4`` do not ask the library where it needs no workspace; the limits are its own."""
+    from fast_route_b200.ops import fp4
+    need = lib.fr_fp4_quantize_workspace_bytes
+    assert need(1, 1, fp4._SMALL) == 0 and need(7, fp4._SMALL // 32, 32) == 0
+    assert need(1, fp4._SMALL // 32 + 1, 32) > 0 and need(7, fp4._SMALL // 32 + 1, 32) > 0
+    for block in (16, 32):
+        for n, k in ((1, 32), (5000, 4096)):
+            need = lib.fr_fp4_gemm_workspace_bytes
+            assert need(1, n, k, block) == need(32, n, k, block) == need(33, n, k, block) == need(128, n, k, block) == 0
+            assert need(129, n, k, block) > 0
