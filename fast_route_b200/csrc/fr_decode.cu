@@ -12,12 +12,15 @@
 //   stream needs no block barriers and runs on across row tiles, across experts and across the grid barrier: the first
 //   weights of w2 are in flight while the last activations are still being written.
 // * The products are mma.sync m16n8k16 with the TOKENS on the 16-row side: 8 weight rows by 16 tokens per instruction
-//   (a tcgen05 tile would be 128 weight rows, too coarse to split a layer of a few thousand rows over 296 CTAs, and
-//   its operand has to pass through shared memory and a barrier).  A lane's 16 bytes are 8 consecutive k of one row;
-//   the dot product does not care about the order of k, so both operands use the same permutation of k and no data is
-//   moved between lanes.
+//   (a tcgen05 tile is 128 weight rows: too coarse to split a layer of a few thousand rows over 296 CTAs; a large layer
+//   has rows enough, but its memory stream is the limit with 16-bit weights, and 4-bit weights would have to be expanded
+//   into shared or tensor memory behind a barrier, or multiplied as they are with tokens in 4-bit terms).
+//   A lane's 16 bytes are 8 consecutive k of one row; the dot product does not care about the order of k, so both
+//   operands use the same permutation of k and no data is moved between lanes.
 // * 4-bit experts are expanded in registers to the exact 16-bit weight (E2M1 * E4M3 has at most six significant bits),
-//   so the arithmetic is that of 16-bit weights.
+//   so the arithmetic is that of 16-bit weights.  No single pipe limits them (1 token of 8 experts: integer pipe active for
+//   41 % of the cycles, FMA 23, tensor 21): 37 instructions per word of eight codes on two warps per scheduler leave
+//   latencies and instruction fetches in the open.
 //
 // The eight warps of a CTA split K; their partial sums meet in shared memory in warp order, so results do not depend
 // on timing.  fp32 accumulation throughout; the activations between the two products are rounded to the 16-bit type.
@@ -69,7 +72,7 @@ struct DecodeParams {
 template <int WF, bool HI>
 struct DecodeCfg {
   static constexpr bool TWO = WF == WF_16BIT;
-  static constexpr int STAGES = 2;                  // FIFO depth (four were 3 % slower: requests queue in the memory system)
+  static constexpr int STAGES = 2;                  // FIFO depth (4-bit: four are 6 to 8 % slower; 16-bit: no room)
   static constexpr int STAGE = TWO ? kDecCodeBytes : kDecCodeBytes + kDecScaleBytes;
   static constexpr int NS2 = 2, LN2 = 2;            // GEMM2: sub-tiles of 8 rows, and 128-byte lines of a row per stage
   static constexpr int TOKENS = HI ? 16 : 8;
@@ -142,7 +145,7 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
 }
 
 // Expansion of a word of eight packed codes to 16-bit numbers: value * block scale / kUnit, exact.  fp16 has a conversion
-// instruction (half the issue slots of the shifts: 4-bit experts of a 1-token layer 104 -> 90 us); bf16 has none.
+// instruction (half the issue slots of the shifts: 4-bit experts of a 1-token layer 94 us in bf16, 76 in fp16); bf16 has none.
 template <bool BF16, int WF>
 struct Fp4Expand {
   // what is left to multiply the sums with: the factors below keep every intermediate inside the 16-bit format
@@ -1046,7 +1049,8 @@ static DecodeWs decode_ws(int64_t M, int H, int I, int E, int topk) {
   return w;
 }
 
-size_t moe_decode_state() { return decode_ws(1, 1, 1, 1, 1).partial; }    // control words and tagged logits: the same for all sizes
+// control words and tagged logits: the same for all sizes
+size_t moe_decode_state() { return decode_ws(1, 1, 1, 1, 1).partial; }
 
 size_t moe_decode_workspace(int64_t M, int H, int I, int E, int topk) {
   if (M <= 0 || M > kDecTokens || H <= 0 || I <= 0 || E <= 0 || topk <= 0 || topk > E) return 0;

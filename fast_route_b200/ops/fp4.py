@@ -86,7 +86,8 @@ def quantize_fp4(x: torch.Tensor, block: int = 16, global_scale: torch.Tensor = 
 
 def dequantize_fp4(q: torch.Tensor, scale: torch.Tensor, global_scale: torch.Tensor = None,
                    dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The numbers that codes and scales stand for, rounded once to ``dtype`` (fp16, bf16 or fp32)."""
+    """The numbers that codes and scales stand for, in ``dtype`` (fp16, bf16 or fp32).  Block 16: scale * global is rounded to
+    fp32, then code times that, then the result to ``dtype``."""
     _lib.require_cuda(q, scale, global_scale)
     shape, dev = q.shape, q.device
     dims = len(shape)
@@ -116,8 +117,8 @@ def matmul_fp4(a_q: torch.Tensor, a_scale: torch.Tensor, b_q: torch.Tensor, b_sc
                a_global: torch.Tensor = None, b_global: torch.Tensor = None, dtype: torch.dtype = torch.bfloat16,
                out: torch.Tensor = None) -> torch.Tensor:
     """``c[m,n] = a[m,k] . b[n,k]^T`` of two quantised matrices of the same block size (``k`` a multiple of 32) on the
-    block-scaled tensor-core instructions, fp32 accumulation, rounded once to ``dtype`` (fp16 or bf16).  ``out`` may have
-    any row pitch."""
+    block-scaled tensor-core instructions: sums in fp32, times the product of the global scales (two fp32 roundings), then
+    rounded to ``dtype`` (fp16 or bf16).  ``out`` (of either type; ``dtype`` is then not looked at) may have any row pitch."""
     _lib.require_cuda(a_q, a_scale, b_q, b_scale, a_global, b_global, out)
     assert a_q.dim() == 2 and b_q.dim() == 2, "codes are [rows, k/2]"
     block = block_of(a_q, a_scale, "a_scale")

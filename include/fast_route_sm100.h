@@ -301,7 +301,8 @@ int fr_w4a16_dequant(const int32_t* qweight, const void* scales, const int32_t* 
  *   operation a single fp32 rounding.  A block that holds an infinity or a NaN gets a NaN scale and zero codes.
  *   cols must be a multiple of block, mats <= 65535; workspace: fr_fp4_quantize_workspace_bytes (0 = none), needed with
  *   own_global only, no initial state.
- * fr_fp4_dequantize: the numbers, rounded to `dtype`; global_scale may be NULL (1). */
+ * fr_fp4_dequantize: the numbers: scale * global rounded to fp32, code times that rounded to fp32, then to `dtype`;
+ *   global_scale may be NULL (1). */
 size_t fr_fp4_quantize_workspace_bytes(int64_t mats, int64_t rows, int64_t cols);
 int fr_fp4_quantize(const void* x, int dtype, int64_t mats, int64_t rows, int64_t cols, int64_t ld_mat, int64_t ld_row,
                     int block, float* global_scale, int own_global, void* q, void* scale, void* workspace,
@@ -310,7 +311,8 @@ int fr_fp4_dequantize(const void* q, const void* scale, const float* global_scal
                       int64_t cols, int block, int dtype, void* out, void* stream);
 
 /* Product of two such matrices, c[m,n] = a_global * b_global * sum_k a[m,k] b[n,k], on the block-scaled tensor-core
- * instructions with fp32 accumulation; c in FR_F16 / FR_BF16 (row pitch ldc), rounded once.  a and b are dense rows as
+ * instructions with fp32 accumulation; the sums times a_global * b_global (an fp32 product) in fp32, then rounded to c's type,
+ * FR_F16 / FR_BF16 (row pitch ldc).  a and b are dense rows as
  * fr_fp4_quantize writes them (mats = 1), both with the same block size; the global scales are one fp32 each on the
  * device, NULL = 1.  k must be a multiple of 32, the codes 16-byte aligned.  A row whose scales hold a NaN gives NaN in
  * its row (column) of c only.  workspace (16-byte aligned, no initial state): fr_fp4_gemm_workspace_bytes, 0 for at
