@@ -205,10 +205,17 @@ struct Fp4Expand {
   }
 };
 
+static __device__ __noinline__ bool mx4_beyond(const uint8_t* scales, int n) {
+  for (int i = 0; i < n; ++i)
+    if (__ldg(scales + i) > Fp4Expand<true, WF_MX4>::kMx4Top) return true;
+  return false;
+}
+
 // sum of n (a multiple of 32) products of E8M0-scaled codes and 16-bit numbers in fp32: for the tiles with scales beyond 2^6
 // (weights of 512 and more), which no trained layer is known to have, so it is short rather than fast (all of a layer in
-// such scales: 1650 us instead of 91 for 1 token of 8 experts, 1880 instead of 158 for 16 tokens of 64; a second factor in
-// the expansion costs everybody 11 to 14 %, behind a branch 4 to 8).
+// such scales: 1690 us instead of 93 for 1 token of 8 experts, 1910 instead of 157 for 16 tokens of 64; a second factor in
+// the expansion costs everybody 11 to 14 %, behind a branch 4 to 8).  It replaces the sums of (row, token) pairs with such a
+// scale only: the others keep their bits whatever the tile's other rows, or the FIFO's places past its end, hold.
 static __device__ __noinline__ float fp4_dot(const uint8_t* codes, const uint8_t* scales, const uint16_t* x, int n) {
   float sum = 0.0f;
   for (int k = 0; k < n; k += 32) {
@@ -817,8 +824,10 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
           if (dots) {
             const int64_t row = static_cast<int64_t>(e) * 2 * p.I + j0 + j;
             const uint16_t* xr = p.x + static_cast<int64_t>(t) * p.H;
-            hg = fp4_dot(p.w1 + row * rb1, p.s1 + row * sb1, xr, p.H);
-            hu = fp4_dot(p.w1 + (row + p.I) * rb1, p.s1 + (row + p.I) * sb1, xr, p.H);
+            if (mx4_beyond(p.s1 + row * sb1, sb1) || mx4_beyond(p.s1 + (row + p.I) * sb1, sb1)) {
+              hg = fp4_dot(p.w1 + row * rb1, p.s1 + row * sb1, xr, p.H);
+              hu = fp4_dot(p.w1 + (row + p.I) * rb1, p.s1 + (row + p.I) * sb1, xr, p.H);
+            }
           }
           const uint32_t v = pack2<BF16>(silu_f(hg) * hu, 0.0f);
           p.act[(static_cast<int64_t>(a) * p.M + t) * p.I + j0 + j] = static_cast<uint16_t>(v);
@@ -986,15 +995,21 @@ __global__ void __launch_bounds__(kDecThreads, (DecodeCfg<WF, HI>::TWO ? 2 : 1))
 #pragma unroll
         for (int w = 0; w < kDecWarps; ++w) v += sm.part[0][w][r * PS + t];
         if (dots) {                // this CTA's double steps of every expert that has the token
-          v = 0.0f;
           constexpr int KS = 128 * LN2 * 2;
-          for (int q = ks * kDecWarps; q < n_active * nb2; q = (q + 1) % kDecWarps ? q + 1 : q + 1 + n2nd - kDecWarps) {
-            const int slot = q / nb2, k = (q - slot * nb2) * KS, e = sm.list[slot];
-            if (!((sm.mask[e] >> t) & 1u)) continue;
-            const int64_t row = static_cast<int64_t>(e) * p.H + r0 + r;
-            v = fmaf(sm.weight[e][t], fp4_dot(p.w2 + row * rb2 + k / 2, p.s2 + row * sb2 + k / 32,
-                                              p.act + (static_cast<int64_t>(slot) * p.M + t) * p.I + k, min(KS, p.I - k)), v);
+          bool beyond = false;
+          float sum = 0.0f;
+          for (int pass = 0; pass < 1 + beyond; ++pass) {       // looks first, adds then
+            for (int q = ks * kDecWarps; q < n_active * nb2; q = (q + 1) % kDecWarps ? q + 1 : q + 1 + n2nd - kDecWarps) {
+              const int slot = q / nb2, k = (q - slot * nb2) * KS, n = min(KS, p.I - k), e = sm.list[slot];
+              if (!((sm.mask[e] >> t) & 1u)) continue;
+              const int64_t row = static_cast<int64_t>(e) * p.H + r0 + r;
+              const uint8_t* scales = p.s2 + row * sb2 + k / 32;
+              if (pass == 0) beyond |= mx4_beyond(scales, n / 32);
+              else sum = fmaf(sm.weight[e][t], fp4_dot(p.w2 + row * rb2 + k / 2, scales,
+                                                       p.act + (static_cast<int64_t>(slot) * p.M + t) * p.I + k, n), sum);
+            }
           }
+          if (beyond) v = sum;
         }
         const int64_t at = static_cast<int64_t>(t) * p.H + r0 + r;
         if (p.ksplit == 1) p.out[at] = static_cast<uint16_t>(pack2<BF16>(v, 0.0f));

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import fast_route_b200 as fr
+from fast_route_b200 import synth
 from oracle import fp4 as o
 
 pytestmark = pytest.mark.gpu
@@ -116,3 +117,28 @@ def test_every_code_with_every_power_of_two_scale(dev):
             # of tiny * eps for each
             bound = (eps + 8 * 2.0 ** -23) * np.abs(want) + tiny * eps
             assert (np.abs(out.cpu().double().numpy() - want) <= bound).all()
+
+
+@pytest.mark.parametrize("M", [6, 13])
+@pytest.mark.parametrize("H,I", [(512, 1408), (320, 2080), (1088, 512)])
+@pytest.mark.parametrize("value", [0xFF, 170, 254])
+def test_scales_beyond_stay_with_their_expert(dev, M, H, I, value):
+    """NaN and large scales in one expert: the tokens that go elsewhere keep every bit, also where row tiles are shared."""
+    E, k = 8, 2
+    x, gate, w1, w2 = (t.to(dev) for t in synth.moe_inputs(M, H, I, E, seed=M + H, dtype=torch.bfloat16, weight_std=0.05))
+    q1, s1, _, q2, s2, _ = fr.quantize_experts_fp4(w1, w2, 32)
+    run = lambda a, b: fr.fused_moe_decode_fp4(x, gate, q1, a, q2, b, k, return_routing=True)  # noqa: E731
+    clean, _, ti = run(s1, s2)
+    victim = int(ti[0, 0])
+    hit = (ti == victim).any(1)
+    assert 0 < int(hit.sum()) < M
+    for which in (0, 1):
+        for rows in (slice(None), slice(3, None, 7)):
+            s = [s1.clone(), s2.clone()]
+            s[which].view(torch.uint8)[victim, rows] = value
+            out = run(*s)[0]
+            assert torch.equal(out[~hit], clean[~hit])
+            assert not torch.equal(out[hit], clean[hit])
+            if which == 1 and rows.step:          # rows of w2 are rows of the output
+                other = [r for r in range(H) if r % 7 != 3]
+                assert torch.equal(out[:, other], clean[:, other])
