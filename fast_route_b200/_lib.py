@@ -159,7 +159,8 @@ _workspaces: dict = {}
 
 def workspace(nbytes: int, device, tag: str = "layer") -> torch.Tensor:
     """A cached, 1024-byte aligned byte buffer per (device, stream, tag); grows on demand.
-    New buffers are zero-filled once (the align stage keeps its grid-barrier words there)."""
+    New buffers are zero-filled once (the align stage keeps its grid-barrier words there).  Layers of several launches
+    meet in it, so of two threads only one at a time may call such a layer on a stream."""
     key = (torch.device(device).index, stream_ptr(device), tag)
     buf = _workspaces.get(key)
     if buf is None or buf.numel() < nbytes + 1024:
